@@ -64,7 +64,8 @@ typedef enum lsc_dtype {
   LSC_DTYPE_U8 = 7,
   LSC_DTYPE_QUINT8 = 8,
   LSC_DTYPE_QINT8 = 9,
-  LSC_DTYPE_QINT32 = 10
+  LSC_DTYPE_QINT32 = 10,
+  LSC_DTYPE_BF16 = 11 /* no counterpart in the reference: lsc_rmsnorm and the paged cache only */
 } lsc_dtype;
 
 /* StorageLayout (lightship.h:90-97; common/types.rs) */
@@ -421,6 +422,102 @@ lsc_status lsc_transpose_heads_f16(const void* x, void* y, int64_t x_batch_strid
  * yields NaN outputs. */
 lsc_status lsc_attention_f16(const void* qkv, int64_t batch, int64_t seq, int64_t heads, float alpha,
                              float* out_f32, int8_t* out_i8, float s_out, int32_t rounding, lsc_stream stream);
+
+/* ---- decoder operators (no counterpart in the reference) ----------------------------------
+ * Root-mean-square norm of the rows of [rows, d], with the residual's addition and an int8
+ * output for the INT8 projection that follows:
+ *   h   = x + residual                          (f32; residual may be NULL: h = x)
+ *   sum_out = h                                 (rounded to residual_dtype; may be NULL)
+ *   y   = h / sqrt(mean(h^2) + eps) * gamma     (gamma [d] f32, NULL = 1; sums in f32)
+ *   out = y                                     (rounded to x_dtype; may be NULL)
+ *   out_i8 = clamp(R(y / s), -128, 127)         (may be NULL; at least one of out / out_i8)
+ * s is s_out (> 0), or, when row_scales is given, the row's own scale max|y| / 127 (1 for a row
+ * of zeros: find_scale_zp's symmetric rule, quantization/helpers.rs:101-136), written to
+ * row_scales[row]; s_out is then not read.  NaN gives the code 0 and does not enter max|y|.
+ * x_dtype F32, F16 or BF16; residual_dtype the same type or F32.  Strides are elements between
+ * rows (>= d); the elements of a row are contiguous.  Any d, strides and alignment to the
+ * element's size; rows that are 16-byte aligned throughout are read as vectors.  sum_out may be
+ * residual or x itself, out may be x itself (same type and stride); no other overlap.  A row
+ * whose sum of squares overflows f32 gives zeros. */
+lsc_status lsc_rmsnorm(const void* x, int32_t x_dtype, int64_t x_stride, const void* residual,
+                       int32_t residual_dtype, int64_t residual_stride, int64_t rows, int64_t d,
+                       const float* gamma, float eps, void* sum_out, int64_t sum_stride, void* out,
+                       int64_t out_stride, int8_t* out_i8, int64_t i8_stride, float s_out, float* row_scales,
+                       int32_t rounding, lsc_stream stream);
+
+/* A paged key-value cache.  Token t of sequence b lives in page page_table[b * table_stride +
+ * t / page_size], slot t % page_size; element (page, slot, head, i) of the keys is at
+ * k + page * page_stride + slot * token_stride + head * head_stride + i (elements), likewise for
+ * the values.  page_table and kv_lens are device memory, read when a kernel runs: kv_lens[b]
+ * counts the tokens of sequence b with the ones that the call appends or asks about among them.
+ * k and v 16-byte aligned, strides multiples of 8 elements; page_size a power of two from 8 to
+ * 256; head_dim 64 or 128; at most 1024 key-value heads and 65535 sequences.
+ * Device data out of range never leads to an access out of range: a length outside
+ * [0, max_pages * page_size] is clamped to it, a page outside [0, num_pages) reads as zeros and
+ * is not written, query offsets that decrease or pass the tokens given make their sequence
+ * empty, and each of these raises the error word that lsc_check_device reports
+ * (LSC_ERROR_EXECUTION_FAILED).  Table entries of pages without a visible key are not read. */
+typedef struct lsc_paged_kv {
+  void* k;
+  void* v;
+  int32_t dtype; /* LSC_DTYPE_F16 or LSC_DTYPE_BF16 */
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int64_t num_pages;
+  int64_t page_stride, token_stride, head_stride;
+  const int32_t* page_table; /* [batch, max_pages] */
+  int64_t table_stride;
+  const int32_t* kv_lens; /* [batch] */
+  int32_t max_pages;
+  int32_t batch;
+} lsc_paged_kv;
+
+/* Writes the new tokens' keys and values into their pages.  Sequence b's new tokens are rows
+ * q_offsets[b] .. q_offsets[b + 1] - 1 of k_new / v_new (device int32 [batch + 1]; `tokens` rows
+ * in all) and take its last places, up to kv_lens[b] - 1; a new token that would come before
+ * place 0 is left out and raises the error word.  Rows before the first offset or behind the
+ * last one are not read.  Row t, head h is at k_new + t * new_token_stride + h * new_head_stride
+ * (elements, multiples of 8; 16-byte aligned bases): the K and V parts of a fused QKV projection
+ * can be given in place. */
+lsc_status lsc_kv_cache_append(const lsc_paged_kv* cache, const void* k_new, const void* v_new, int64_t tokens,
+                               int64_t new_token_stride, int64_t new_head_stride, const int32_t* q_offsets,
+                               lsc_stream stream);
+
+/* Causal attention of a ragged batch of new tokens over the cache they were appended to.  Query
+ * head h of row t (q + t * q_token_stride + h * q_head_stride, elements, multiples of 8, base
+ * 16-byte aligned, the cache's type) reads key-value head h / (q_heads / kv_heads).  The rows of
+ * sequence b are q_offsets[b] .. q_offsets[b + 1] - 1 and stand at its last positions
+ * (p = kv_lens[b] - count + i).  Key j is visible at position p iff
+ *   j <= p  and  (window == 0  or  j > p - window  or  j < sinks):
+ * with window > 0 a sliding window of that many tokens, beside which the sequence's first `sinks`
+ * tokens stay visible.  A row that sees no key (p < 0) gives zeros.
+ *   out[t, h, :] = softmax_j(alpha * q . k_j) v_j       alpha > 0
+ * Scores, maxima and sums in f32; probabilities are rounded to the cache's type for the second
+ * product, as are the values they weigh.  out [tokens, q_heads, head_dim] contiguous in the
+ * cache's type and/or out_i8 of that shape, quantized per tensor with s_out (`rounding` as
+ * lsc_rounding); 16-byte aligned.  Rows before the first offset or behind the last one are left
+ * as they are.  What the cache holds behind a sequence's last token has no effect.  Rows are
+ * worked on in blocks of at most 256 (row, head) pairs of one sequence and key-value head: a place
+ * that no row of a block sees has no effect on it, whatever it holds, but a value in V that is not
+ * finite reaches every row of a block that has a row which sees it. */
+lsc_status lsc_paged_attention_prefill(const lsc_paged_kv* cache, const void* q, int64_t tokens, int32_t q_heads,
+                                       int64_t q_token_stride, int64_t q_head_stride, const int32_t* q_offsets,
+                                       float alpha, int64_t window, int64_t sinks, void* out, int8_t* out_i8,
+                                       float s_out, int32_t rounding, lsc_stream stream);
+
+/* The same for one new token per sequence (row b of q [batch, q_heads, head_dim] at position
+ * kv_lens[b] - 1; an empty sequence gives zeros): the cache's length is split over the GPU and
+ * the parts are joined in a fixed order, so results do not change from run to run.  Places that
+ * the row does not see have no effect, whatever they hold.  `workspace`: device scratch of
+ * lsc_paged_attention_decode_workspace_size(cache, q_heads) bytes, 16-byte aligned, with any
+ * content; calls that share one must be ordered on one stream (two captured graphs that share
+ * one must not run at the same time). */
+uint64_t lsc_paged_attention_decode_workspace_size(const lsc_paged_kv* cache, int32_t q_heads);
+lsc_status lsc_paged_attention_decode(const lsc_paged_kv* cache, const void* q, int32_t q_heads,
+                                      int64_t q_token_stride, int64_t q_head_stride, float alpha, int64_t window,
+                                      int64_t sinks, void* out, int8_t* out_i8, float s_out, int32_t rounding,
+                                      void* workspace, uint64_t workspace_bytes, lsc_stream stream);
 
 /* ---- models and sessions (ONNX; FP32 NCHW graphs) ----------------------------------------
  * An ONNX model loaded from memory (LightShipEngine_LoadModelFromMemory, lightship.h:186-198;

@@ -28,7 +28,7 @@ ERROR_UNSUPPORTED_LAYOUT = 14
 ERROR_TIMEOUT = 15
 
 ACT_NONE, ACT_RELU, ACT_RELU6, ACT_SILU, ACT_GELU = 0, 1, 2, 3, 4
-DTYPE_F32, DTYPE_F16 = 0, 1  # lsc_dtype
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 11  # lsc_dtype
 ROUND_HALF_AWAY, ROUND_HALF_EVEN = 0, 1
 FP32_3XTF32, FP32_TF32, FP32_WINOGRAD = 0, 1, 2
 MEM_HOST, MEM_DEVICE = 0, 1
@@ -87,6 +87,14 @@ class lsc_memory_block(C.Structure):
                 ("alignment", C.c_uint64), ("location", C.c_int32)]
 
 
+class lsc_paged_kv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("num_pages", C.c_int64),
+                ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("kv_lens", C.c_void_p),
+                ("max_pages", C.c_int32), ("batch", C.c_int32)]
+
+
 P = C.c_void_p
 I32 = C.c_int32
 I64 = C.c_int64
@@ -136,6 +144,13 @@ SIGNATURES = {
                                   I64, I64, I64, P]),
     "lsc_transpose_heads_f16": (ST, [P, P, I64, I64, I64, I64, I64, I64, I64, I64, P]),
     "lsc_attention_f16": (ST, [P, I64, I64, I64, F32, P, P, F32, I32, P]),
+    "lsc_rmsnorm": (ST, [P, I32, I64, P, I32, I64, I64, I64, P, F32, P, I64, P, I64, P, I64, F32, P, I32, P]),
+    "lsc_kv_cache_append": (ST, [C.POINTER(lsc_paged_kv), P, P, I64, I64, I64, P, P]),
+    "lsc_paged_attention_prefill": (ST, [C.POINTER(lsc_paged_kv), P, I64, I32, I64, I64, P, F32, I64, I64, P, P,
+                                         F32, I32, P]),
+    "lsc_paged_attention_decode_workspace_size": (C.c_uint64, [C.POINTER(lsc_paged_kv), I32]),
+    "lsc_paged_attention_decode": (ST, [C.POINTER(lsc_paged_kv), P, I32, I64, I64, F32, I64, I64, P, P, F32, I32, P,
+                                        C.c_uint64, P]),
     "lsc_model_load_onnx": (ST, [C.c_char_p, C.c_uint64, C.POINTER(P)]),
     "lsc_model_destroy": (None, [P]),
     "lsc_model_info": (ST, [P, C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),

@@ -136,3 +136,75 @@ def attention_f16(qkv, batch, seq, heads, alpha=0.125, out_f32=None, out_i8=None
             raise ValueError(f"attention_f16: {name} too small")
     check(lib().lsc_attention_f16(_ptr(qkv), batch, seq, heads, float(alpha), _ptr(out_f32), _ptr(out_i8),
                                   float(s_out), int(rounding), _stream(qkv.device)))
+
+
+_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+def _rows(t, dtype, name, like=None):
+    """A CUDA tensor of rows whose elements are contiguous: (pointer, row stride)."""
+    if t is None:
+        return None, 0
+    if t.dim() != 2 or not t.is_cuda or t.dtype != dtype or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: expected a 2-D CUDA {dtype} tensor with contiguous rows, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}, strides {t.stride()}")
+    if like is not None and (t.shape != like.shape or t.device != like.device):
+        raise ValueError(f"{name}: shape {tuple(t.shape)} on {t.device} does not match {tuple(like.shape)} on "
+                         f"{like.device}")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def rmsnorm(x, gamma=None, eps=1e-5, residual=None, sum_out=None, out=None, out_i8=None, s_out=0.0,
+            row_scales=None, rounding=_lib.ROUND_HALF_AWAY):
+    """Root-mean-square norm of the rows of ``x`` (see ``lsc_rmsnorm``): h = x + residual,
+    y = h / sqrt(mean(h^2) + eps) * gamma.
+
+    x: [rows, d] f32, f16 or bf16 with contiguous rows; residual: the same shape, x's type or f32;
+    gamma: [d] f32.  Writes ``sum_out`` = h (the residual's type), ``out`` = y (x's type) and
+    ``out_i8`` = y quantized with ``s_out``, or with each row's max|y| / 127 when ``row_scales``
+    ([rows] f32) is given to receive them.  With neither ``out`` nor ``out_i8``, ``out`` is
+    allocated.  Returns ``out`` if there is one, else ``out_i8``.
+    """
+    code = _DTYPES.get(x.dtype)
+    if code is None:
+        raise ValueError(f"x: expected f32, f16 or bf16, got {x.dtype}")
+    px, sx = _rows(x, x.dtype, "x")
+    if out is None and out_i8 is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    rcode = code
+    if residual is not None:
+        if residual.dtype != x.dtype and residual.dtype != torch.float32:
+            raise ValueError(f"residual: expected {x.dtype} or f32, got {residual.dtype}")
+        rcode = _DTYPES[residual.dtype]
+    pr, sr = _rows(residual, None if residual is None else residual.dtype, "residual", x)
+    ps, ss = _rows(sum_out, x.dtype if residual is None else residual.dtype, "sum_out", x)
+    po, so = _rows(out, x.dtype, "out", x)
+    pq, sq = _rows(out_i8, torch.int8, "out_i8", x)
+    rows, d = x.shape
+    for name, t, n in (("gamma", gamma, d), ("row_scales", row_scales, rows)):
+        if t is not None:
+            _need(t, torch.float32, name)
+            if t.numel() != n or t.device != x.device:
+                raise ValueError(f"{name}: expected {n} values on {x.device}")
+    with _on(x.device):
+        check(lib().lsc_rmsnorm(px, code, sx, pr, rcode, sr, rows, d, _ptr(gamma), float(eps), ps, ss, po, so, pq, sq,
+                                float(s_out), _ptr(row_scales), int(rounding), _stream(x.device)))
+    return out if out is not None else out_i8
+
+
+class _Here:
+    """No device change."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _on(device):
+    """Makes ``device`` the current one for the call, as the library expects."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
