@@ -3,45 +3,16 @@
 //   O[t, h, :] = sum_j P[t, j] V[j, :],  P = softmax_j(alpha * Q[t, h, :] . K[j, :]) over the visible j
 // One warp per (row, query head) walks the visible keys with the running maximum m and sum l of
 // the softmax: a new score s rescales the sum and the output by exp(m - max(m, s)).
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
-#include "epilogue.cuh"
-#include "paged_cache.cuh"
+#include "attention_paged.cuh"
 
 namespace lsc {
-float reciprocal_or_zero(float s);
 namespace {
-
-struct AttnArgs {
-  const uint16_t* q;
-  int64_t tokens, q_token, q_head;
-  const int32_t* offsets;  // null: row b is sequence b's one new token
-  int32_t q_heads, group;
-  float alpha;
-  int32_t window, sinks;
-  uint16_t* out;
-  int8_t* out_i8;
-  float s_out, inv_s_out;
-  int32_t rounding;
-};
 
 template <bool BF16>
 __device__ __forceinline__ float2 to_f32(uint32_t v) {
   if constexpr (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
   else return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
-template <bool BF16>
-__device__ __forceinline__ uint32_t to_16(float a, float b) {
-  if constexpr (BF16) {
-    const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&r);
-  } else {
-    const __half2 r = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-}
-
 template <bool BF16, int D>
 __global__ void __launch_bounds__(128) paged_attention_kernel(const PagedView c, const AttnArgs a) {
   constexpr int W = D / 64;  // 32-bit words of a row per lane
@@ -98,10 +69,10 @@ __global__ void __launch_bounds__(128) paged_attention_kernel(const PagedView c,
       }
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      s *= a.alpha;
+      s *= a.scale_log2;
       const float m_new = s > m ? s : m;
       const float ref = m_new == -INFINITY ? 0.0f : m_new;
-      const float f = expf(m - ref), e = expf(s - ref);
+      const float f = ex2_approx(m - ref), e = ex2_approx(s - ref);
       m = m_new;
       l = l * f + e;
 #pragma unroll
@@ -116,7 +87,7 @@ __global__ void __launch_bounds__(128) paged_attention_kernel(const PagedView c,
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const float x = o[w].x * inv, y = o[w].y * inv;
-      if (a.out) *reinterpret_cast<uint32_t*>(a.out + at + 2 * w) = to_16<BF16>(x, y);
+      if (a.out) *reinterpret_cast<uint32_t*>(a.out + at + 2 * w) = pack16<BF16>(x, y);
       if (a.out_i8) {
         if (a.rounding == LSC_ROUND_HALF_EVEN) {
           a.out_i8[at + 2 * w] = static_cast<int8_t>(requant_i8<LSC_ROUND_HALF_EVEN>(x, a.s_out));
@@ -130,7 +101,25 @@ __global__ void __launch_bounds__(128) paged_attention_kernel(const PagedView c,
   }
 }
 
-// The checks that both entry points share.
+lsc_status launch_simple(const lsc_paged_kv* cache, const DeviceState* ds, const PagedView& c, const AttnArgs& a,
+                         cudaStream_t st) {
+  const int64_t ctas = (a.tokens * a.q_heads + 3) / 4;
+  const int64_t cap = static_cast<int64_t>(ds->sm_count) * 64;
+  const int grid = static_cast<int>(ctas < cap ? ctas : cap);
+  const bool bf16 = cache->dtype == LSC_DTYPE_BF16;
+  if (cache->head_dim == 64) {
+    if (bf16) paged_attention_kernel<true, 64><<<grid, 128, 0, st>>>(c, a);
+    else paged_attention_kernel<false, 64><<<grid, 128, 0, st>>>(c, a);
+  } else {
+    if (bf16) paged_attention_kernel<true, 128><<<grid, 128, 0, st>>>(c, a);
+    else paged_attention_kernel<false, 128><<<grid, 128, 0, st>>>(c, a);
+  }
+  LSC_CUDA_TRY(cudaGetLastError());
+  return LSC_SUCCESS;
+}
+
+}  // namespace
+
 lsc_status attention_args(const lsc_paged_kv* cache, const char* who, const void* q, int64_t tokens, int32_t q_heads,
                           int64_t q_token, int64_t q_head, float alpha, int64_t window, int64_t sinks, void* out,
                           int8_t* out_i8, float s_out, int32_t rounding, AttnArgs* a) {
@@ -138,7 +127,7 @@ lsc_status attention_args(const lsc_paged_kv* cache, const char* who, const void
   if (q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads)
     return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: %d query heads are not a multiple of %d key-value heads", who,
                      q_heads, cache->kv_heads);
-  if (!(alpha > 0.0f) || !(alpha <= 3.0e38f))
+  if (!(alpha > 0.0f) || !(alpha <= 1.0e38f))
     return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: alpha must be positive and finite", who);
   if (window < 0 || sinks < 0) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: negative window or sinks", who);
   if (rounding != LSC_ROUND_HALF_AWAY && rounding != LSC_ROUND_HALF_EVEN)
@@ -161,7 +150,7 @@ lsc_status attention_args(const lsc_paged_kv* cache, const char* who, const void
   a->q_head = q_head;
   a->q_heads = q_heads;
   a->group = q_heads / cache->kv_heads;
-  a->alpha = alpha;
+  a->scale_log2 = alpha * kLog2e;
   // positions stay below 2^30: a longer window is no window, more sinks see no more
   a->window = static_cast<int32_t>(window > (1 << 30) ? 0 : window);
   a->sinks = static_cast<int32_t>(window == 0 ? 0 : (sinks > (1 << 30) ? (1 << 30) : sinks));
@@ -174,24 +163,19 @@ lsc_status attention_args(const lsc_paged_kv* cache, const char* who, const void
   return LSC_SUCCESS;
 }
 
-lsc_status launch_simple(const lsc_paged_kv* cache, const DeviceState* ds, const PagedView& c, const AttnArgs& a,
-                         cudaStream_t st) {
-  const int64_t ctas = (a.tokens * a.q_heads + 3) / 4;
-  const int64_t cap = static_cast<int64_t>(ds->sm_count) * 64;
-  const int grid = static_cast<int>(ctas < cap ? ctas : cap);
-  const bool bf16 = cache->dtype == LSC_DTYPE_BF16;
-  if (cache->head_dim == 64) {
-    if (bf16) paged_attention_kernel<true, 64><<<grid, 128, 0, st>>>(c, a);
-    else paged_attention_kernel<false, 64><<<grid, 128, 0, st>>>(c, a);
-  } else {
-    if (bf16) paged_attention_kernel<true, 128><<<grid, 128, 0, st>>>(c, a);
-    else paged_attention_kernel<false, 128><<<grid, 128, 0, st>>>(c, a);
-  }
-  LSC_CUDA_TRY(cudaGetLastError());
-  return LSC_SUCCESS;
+lsc_status paged_tensor_map(CUtensorMap* map, const lsc_paged_kv* cache, const PagedView& view, const void* base,
+                            uint32_t box_rows) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(cache->head_dim), static_cast<uint64_t>(cache->page_size),
+                            static_cast<uint64_t>(cache->kv_heads), static_cast<uint64_t>(cache->num_pages)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(view.token_stride) * 2, static_cast<uint64_t>(view.head_stride) * 2,
+                               static_cast<uint64_t>(view.page_stride) * 2};
+  const uint32_t box[4] = {64, box_rows, 1, 1};
+  const uint32_t ones[4] = {1, 1, 1, 1};
+  return encode_tmap_4d(map, cache->dtype == LSC_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        base, dims, strides, box, ones, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-}  // namespace
 }  // namespace lsc
 
 using namespace lsc;
@@ -213,31 +197,6 @@ lsc_status lsc_paged_attention_prefill(const lsc_paged_kv* cache, const void* q,
   if (tokens == 0 || c.batch == 0) return LSC_SUCCESS;
   if (!q_offsets) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: null offsets", who);
   a.offsets = q_offsets;
-  DeviceState* ds = nullptr;
-  if ((st = paged_device(who, &ds, &c))) return st;
-  return launch_simple(cache, ds, c, a, static_cast<cudaStream_t>(stream));
-}
-
-uint64_t lsc_paged_attention_decode_workspace_size(const lsc_paged_kv* cache, int32_t q_heads) {
-  return cache && q_heads > 0 ? 16 : 0;
-}
-
-lsc_status lsc_paged_attention_decode(const lsc_paged_kv* cache, const void* q, int32_t q_heads,
-                                      int64_t q_token_stride, int64_t q_head_stride, float alpha, int64_t window,
-                                      int64_t sinks, void* out, int8_t* out_i8, float s_out, int32_t rounding,
-                                      void* workspace, uint64_t workspace_bytes, lsc_stream stream) {
-  const char* who = "paged_attention_decode";
-  PagedView c;
-  AttnArgs a;
-  lsc_status st = paged_view(cache, who, &c);
-  if (st) return st;
-  st = attention_args(cache, who, q, c.batch, q_heads, q_token_stride, q_head_stride, alpha, window, sinks, out, out_i8,
-                      s_out, rounding, &a);
-  if (st) return st;
-  if (c.batch == 0) return LSC_SUCCESS;
-  if (!workspace || workspace_bytes < lsc_paged_attention_decode_workspace_size(cache, q_heads) ||
-      (reinterpret_cast<uintptr_t>(workspace) & 15))
-    return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: the workspace is missing, too small or not 16-byte aligned", who);
   DeviceState* ds = nullptr;
   if ((st = paged_device(who, &ds, &c))) return st;
   return launch_simple(cache, ds, c, a, static_cast<cudaStream_t>(stream));

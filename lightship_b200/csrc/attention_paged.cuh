@@ -1,0 +1,67 @@
+// attention_paged.cuh -- what the two attention kernels over the paged cache share: arguments,
+// 16-bit packing, and which key tiles a range of query positions meets.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "epilogue.cuh"
+#include "paged_cache.cuh"
+
+namespace lsc {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttnArgs {
+  const uint16_t* q;
+  int64_t tokens, q_token, q_head;
+  const int32_t* offsets;  // null: row b is sequence b's one new token
+  int32_t q_heads, group;
+  float scale_log2;  // alpha * log2(e): scores are kept as powers of two
+  int32_t window, sinks;
+  uint16_t* out;
+  int8_t* out_i8;
+  float s_out, inv_s_out;
+  int32_t rounding;
+};
+
+// The checks that both entry points share; fills `a` but for the offsets.
+lsc_status attention_args(const lsc_paged_kv* cache, const char* who, const void* q, int64_t tokens, int32_t q_heads,
+                          int64_t q_token, int64_t q_head, float alpha, int64_t window, int64_t sinks, void* out,
+                          int8_t* out_i8, float s_out, int32_t rounding, AttnArgs* a);
+
+// Tensor map of the keys or values {head_dim, page_size, heads, pages}, boxes of 64 x rows.
+lsc_status paged_tensor_map(CUtensorMap* map, const lsc_paged_kv* cache, const PagedView& view, const void* base,
+                            uint32_t box_rows);
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// {lo, hi} rounded to the cache's type and packed
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t d;
+  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
+// The key tiles (of TILE places) that queries at positions first .. last meet, sinks apart from
+// the window: tile i of n is key tile i < sink_tiles ? i : start + i - sink_tiles.
+template <int TILE>
+struct TileList {
+  int32_t n, sink_tiles, start;
+  __device__ __forceinline__ TileList(int32_t first, int32_t last, int32_t window, int32_t sinks) {
+    const int32_t low = window > 0 && first >= window ? first - window + 1 : 0;
+    const int32_t kept = sinks < low ? sinks : low;
+    sink_tiles = (kept + TILE - 1) / TILE;
+    start = low / TILE;
+    if (start <= sink_tiles) sink_tiles = start = 0;
+    n = last < 0 ? 0 : sink_tiles + last / TILE + 1 - start;
+  }
+  __device__ __forceinline__ int32_t tile(int32_t i) const { return i < sink_tiles ? i : start + i - sink_tiles; }
+};
+
+}  // namespace lsc

@@ -24,6 +24,7 @@ lsc_status paged_view(const lsc_paged_kv* c, const char* who, PagedView* view) {
     return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: null page table or lengths", who);
   if (c->batch > 1 && c->table_stride < c->max_pages)
     return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: the page table's rows overlap", who);
+  if (c->batch > 0 && c->num_pages < 1) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: a cache without pages", who);
   if (c->num_pages > 0 && (!c->k || !c->v)) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: null cache", who);
   if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
     return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: k and v must be 16-byte aligned", who);
