@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
       int32_t page = page_of(cur.i);
       for (int32_t i = cur.i; i < cur.i + count; ++i) {
         const int32_t next = i + 1 < cur.i + count ? page_of(i + 1) : 0;
-        if (!(ok = mbar_wait(empty + stage, phase ^ 1u, abort_flag, c.err))) break;
+        if (!(ok = warp_wait(empty + stage, phase ^ 1u, abort_flag, c.err))) break;
         if (lane == 0) mbar_arrive_expect_tx(full + stage, 2 * Shape::kTileBytes);
         __syncwarp();
         if (lane < boxes) {
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
     for (int32_t i = cur.i; i < cur.i + count; ++i) {
-      if (!mbar_wait(full + stage, phase, abort_flag, c.err)) return;
+      if (!warp_wait(full + stage, phase, abort_flag, c.err)) return;
       const uint32_t sk = smem_u32(smem + 2 * stage * Shape::kTileBytes);
       const uint32_t sv = sk + Shape::kTileBytes;
       const int32_t t0 = cur.tiles.tile(i) * kTile + slice * kKeys;  // this warp's first place
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
     auto swap_sync = [&]() -> bool {
       __syncwarp();
       if (lane == 0) mbar_arrive(swap_bar);
-      const bool ok = mbar_wait(swap_bar, swap_phase, abort_flag, c.err);
+      const bool ok = warp_wait(swap_bar, swap_phase, abort_flag, c.err);
       swap_phase ^= 1u;
       return ok;
     };

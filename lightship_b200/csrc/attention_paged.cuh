@@ -39,6 +39,11 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
+// mbar_wait by all lanes of a warp with one outcome (false for all when it ran out for one).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err)) != 0;
+}
+
 // {lo, hi} rounded to the cache's type and packed
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {

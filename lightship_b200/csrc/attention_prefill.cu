@@ -1,0 +1,748 @@
+// attention_prefill.cu -- causal attention of a ragged batch of new tokens over the paged key-value
+// cache, with a sliding window and sinks, on the 5th-generation tensor cores:
+//   O[t, h, :] = sum_j p_j V[j, :] / l,  p_j = 2^(s_j - m),  s_j = alpha log2(e) Q[t, h, :] . K[j, :]
+// over the visible places j of the row's sequence, in one pass over the keys with a running
+// reference m and sum l.
+//
+// A unit of work is up to 256 rows, two tiles of 128: consecutive tokens of one sequence times the
+// query heads that share a key-value head (hp of them), so a tile of K and V is read once for all
+// of them and all heads of a token share one mask.  One persistent CTA per SM walks the units,
+// those at the highest positions first (they meet the most keys) and turning at each end of the
+// grid, which spreads the causal triangle evenly:
+//   warps 0-3, 4-7  softmax of row tile 0 and 1: thread = row.  S (128 keys) comes from TMEM into
+//                   registers, p goes back to TMEM, packed, in place of S;
+//   warp 8          issues the products: S = Q K^T (A and B in shared memory) and O += P V (A in
+//                   TMEM, V MN-major), the two row tiles in turn, so that one tile's softmax runs
+//                   beside the other's products;
+//   warp 9          brings Q and the K and V tiles by TMA, page by page (boxes of pages without a
+//                   visible place read out of the tensor's range: zeros, no traffic);
+//   warp 10         zeroes the rows of V that no row of the unit sees (a product with p = 0 would
+//                   keep a NaN), in the few tiles that have such rows, before they are released;
+//   warp 11         finds the units.
+// m moves only when a row's maximum passes it by more than 2^8: until then p stays below 2^8,
+// which the 16-bit types and the f32 sums hold as exactly as values below 1, and O needs no
+// rescaling.  When it moves, the softmax thread rescales its row of O in TMEM; the products into O
+// that it follows are complete, because S of this tile was issued behind them.
+// Every wait is bounded (a timeout flags the device error word and ends the CTA's work).
+#include "attention_paged.cuh"
+
+namespace lsc {
+namespace {
+
+constexpr int kTile = 128;            // rows of a row tile, places of a key tile
+constexpr int kPrefillThreads = 384;
+constexpr int kSchedSlots = 4;
+constexpr float kMoveBy = 8.0f;       // log2 of how far a maximum may pass the reference
+
+template <int D>
+struct PrefillShape {
+  static constexpr int kTileBytes = kTile * D * 2;    // Q, K or V of one tile
+  static constexpr int kStages = D == 128 ? 5 : 8;    // K and V tiles in turn
+  static constexpr int kBarBytes = 512;
+  static constexpr int kSmem = (2 + kStages) * kTileBytes + kBarBytes + 1024;
+  static constexpr uint32_t kColS = 0, kColO = 256;   // TMEM columns: S of both tiles, then O of both
+};
+static_assert(PrefillShape<128>::kSmem <= 232448 && PrefillShape<64>::kSmem <= 232448, "shared memory budget");
+
+struct PrefillArgs {
+  AttnArgs a;
+  int32_t hp;          // query heads of a tile
+  int32_t tpt;         // tokens of a tile: 128 / hp
+  int32_t unit_tokens; // tokens of a unit: tpt or 2 tpt
+  int32_t pairs;       // key-value heads x (group / hp)
+};
+
+// A unit: tokens [row0, row0 + count) of the batch, the first at position pos0 of sequence b.
+struct Unit {
+  int32_t b, row0, count, pos0, kvh, head0;
+};
+
+// What the rows of tile w of a unit see.
+struct TileRows {
+  int32_t count, first, last, low;
+  __device__ __forceinline__ TileRows(const PrefillArgs& p, const Unit& u, int w) {
+    count = u.count - w * p.tpt;
+    count = count < 0 ? 0 : (count > p.tpt ? p.tpt : count);
+    first = u.pos0 + w * p.tpt;
+    last = first + count - 1;
+    low = p.a.window > 0 && first >= p.a.window ? first - p.a.window + 1 : 0;
+  }
+  __device__ __forceinline__ bool meets(int32_t tile, int32_t sinks) const {
+    const int32_t j0 = tile * kTile;
+    return count > 0 && j0 <= last && (j0 + kTile > low || j0 < sinks);
+  }
+};
+
+// The units of this CTA, found by one warp.  Sequence b's units stand at levels
+// base_b .. base_b + n_b - 1 (its position in units); F(t) counts those at level t or above.
+struct Scheduler {
+  const PagedView& c;
+  const PrefillArgs& p;
+  int lane;
+  int64_t total;
+  int32_t top;
+  __device__ __forceinline__ void of(int b, int32_t& begin, int32_t& n, int32_t& base, int32_t& count,
+                                     int32_t& len) const {
+    int32_t end;
+    query_rows(p.a.offsets, b, p.a.tokens, c.err, false, begin, end);
+    len = paged_len(c, b, false);
+    count = end - begin;
+    n = (count + p.unit_tokens - 1) / p.unit_tokens;
+    base = len > count ? (len - count) / p.unit_tokens : 0;
+  }
+  __device__ __forceinline__ int64_t at_or_above(int32_t t) const {
+    int64_t f = 0;
+    for (int b = lane; b < c.batch; b += 32) {
+      int32_t begin, n, base, count, len;
+      of(b, begin, n, base, count, len);
+      const int32_t x = base + n - t;
+      f += x < 0 ? 0 : (x > n ? n : x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
+    return f;
+  }
+  __device__ __forceinline__ Scheduler(const PagedView& c_, const PrefillArgs& p_, int lane_)
+      : c(c_), p(p_), lane(lane_), top(0) {
+    for (int b = lane; b < c.batch; b += 32) {
+      int32_t begin, n, base, count, len;
+      of(b, begin, n, base, count, len);
+      top = n > 0 && base + n > top ? base + n : top;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const int32_t other = __shfl_xor_sync(0xffffffffu, top, o);
+      top = other > top ? other : top;
+    }
+    total = at_or_above(0) * p.pairs;
+  }
+  // Unit number i (all lanes)
+  __device__ __forceinline__ Unit find(int64_t i) const {
+    const int64_t u = i / p.pairs;
+    const int32_t pair = static_cast<int32_t>(i - u * p.pairs);
+    int32_t lo = 0, hi = top;  // F(lo) > u >= F(hi)
+    int64_t above = 0;         // F(hi)
+    while (hi - lo > 1) {
+      const int32_t mid = lo + (hi - lo) / 2;
+      const int64_t f = at_or_above(mid);
+      if (f > u) {
+        lo = mid;
+      } else {
+        hi = mid;
+        above = f;
+      }
+    }
+    // the (u - F(lo + 1))-th sequence with a unit at level lo
+    int32_t k = static_cast<int32_t>(u - above);
+    Unit r{};
+    for (int b0 = 0; b0 < c.batch; b0 += 32) {
+      int32_t begin = 0, n = 0, base = 0, count = 0, len = 0;
+      if (b0 + lane < c.batch) of(b0 + lane, begin, n, base, count, len);
+      const bool here = base <= lo && lo < base + n;
+      const uint32_t mask = __ballot_sync(0xffffffffu, here);
+      const int have = __popc(mask);
+      if (k >= have) {
+        k -= have;
+        continue;
+      }
+      const int src = __fns(mask, 0, k + 1);
+      const int32_t first = (lo - base) * p.unit_tokens;
+      r.b = b0 + src;
+      r.row0 = __shfl_sync(0xffffffffu, begin + first, src);
+      r.count = __shfl_sync(0xffffffffu, count - first < p.unit_tokens ? count - first : p.unit_tokens, src);
+      r.pos0 = __shfl_sync(0xffffffffu, len - count + first, src);
+      break;
+    }
+    const int32_t per_head = p.pairs / c.kv_heads;
+    r.kvh = pair / per_head;
+    r.head0 = r.kvh * p.a.group + (pair - r.kvh * per_head) * p.hp;
+    return r;
+  }
+};
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(kPrefillThreads, 1)
+    paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                         const __grid_constant__ CUtensorMap tm_v, const PagedView c, const PrefillArgs p) {
+  using Shape = PrefillShape<D>;
+  constexpr int kBlocks = D / 64;
+  constexpr int kStages = Shape::kStages;
+  constexpr int kBlockBytes = kTile * 128;  // 128 rows of one 128-byte column block
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
+  uint8_t* s_q = smem;
+  uint8_t* s_kv = smem + 2 * Shape::kTileBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_kv + kStages * Shape::kTileBytes);
+  uint64_t* kv_full = bars;
+  uint64_t* kv_empty = kv_full + kStages;
+  uint64_t* landed = kv_empty + kStages;  // V tiles that the zeroing warp passes on
+  uint64_t* q_full = landed + kStages;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* drain = o_full + 2;
+  uint64_t* sched_full = drain + 1;
+  uint64_t* sched_empty = sched_full + kSchedSlots;
+  Unit* sched = reinterpret_cast<Unit*>(sched_empty + kSchedSlots);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sched + kSchedSlots);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const AttnArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(kv_full + s, 1);
+      mbar_init(kv_empty + s, 2);
+      mbar_init(landed + s, 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(s_full + w, 1);
+      mbar_init(p_full + w, 4);
+      mbar_init(o_full + w, 1);
+    }
+    mbar_init(drain, 1);
+    for (int s = 0; s < kSchedSlots; ++s) {
+      mbar_init(sched_full + s, 1);
+      mbar_init(sched_empty + s, 11);  // eight softmax warps, products, loads, zeroing
+    }
+    *abort_flag = 0u;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // The next unit of this CTA for one warp; false when there is none (or after a timeout).
+  uint32_t sched_at = 0, sched_phase = 0;
+  auto next_unit = [&](Unit& u) -> bool {
+    if (!warp_wait(sched_full + sched_at, sched_phase, abort_flag, c.err)) return false;
+    u = sched[sched_at];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sched_empty + sched_at);
+    if (++sched_at == kSchedSlots) {
+      sched_at = 0;
+      sched_phase ^= 1u;
+    }
+    return u.b >= 0;
+  };
+  auto tiles_of = [&](const Unit& u) { return TileList<kTile>(u.pos0, u.pos0 + u.count - 1, a.window, a.sinks); };
+
+  if (warp >= 8) {
+    regs_shrink<88>();
+    if (warp == 11) {
+      // ------------------------------------------------------------------ scheduler
+      if (blockIdx.x == 0) {
+        int32_t begin, end;
+        for (int b = lane; b < c.batch; b += 32) {
+          query_rows(a.offsets, b, a.tokens, c.err, true, begin, end);
+          paged_len(c, b, true);
+        }
+      }
+      const Scheduler s(c, p, lane);
+      bool ok = true;
+      for (int64_t k = 0; ok; ++k) {
+        const int64_t i = k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        Unit u{};
+        u.b = -1;
+        const bool more = k * gridDim.x < s.total;
+        if (more && i >= s.total) continue;  // this round's part is missing; the last round
+        if (more) u = s.find(i);
+        if (!(ok = warp_wait(sched_empty + sched_at, sched_phase ^ 1u, abort_flag, c.err))) break;
+        if (lane == 0) {
+          sched[sched_at] = u;
+          mbar_arrive(sched_full + sched_at);
+        }
+        __syncwarp();
+        if (++sched_at == kSchedSlots) {
+          sched_at = 0;
+          sched_phase ^= 1u;
+        }
+        if (!more) break;
+      }
+    } else if (warp == 9) {
+      // ------------------------------------------------------------------ loads (whole warp)
+      const int page_size = 1 << c.page_shift;
+      const int box_rows = page_size < kTile ? page_size : kTile;
+      const int per_tile = kTile / box_rows;
+      const int boxes = per_tile * kBlocks;  // at most 32
+      const int sub = lane % per_tile, block = lane / per_tile;
+      uint32_t stage = 0, phase = 0, q_phase = 0;
+      uint32_t by_landed = 0, land_parity = 0;  // per stage: how its last tile came, uses of `landed` mod 2
+      int issued = 0, q_loads = 0;
+      bool ok = true;
+      Unit u;
+      while (ok && next_unit(u)) {
+        const TileList<kTile> tiles = tiles_of(u);
+        if (tiles.n == 0) continue;
+        const int32_t last = u.pos0 + u.count - 1;
+        const int32_t low = a.window > 0 && u.pos0 >= a.window ? u.pos0 - a.window + 1 : 0;
+        if (!(ok = warp_wait(q_empty, q_phase ^ 1u, abort_flag, c.err))) break;
+        q_phase ^= 1u;
+        if (lane == 0) {
+          const int q_tiles = u.count > p.tpt ? 2 : 1;
+          mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(q_tiles * kBlocks * p.hp * p.tpt * 128));
+          for (int w = 0; w < q_tiles; ++w)
+            for (int x = 0; x < kBlocks; ++x)
+              tma_load_3d(&tm_q, q_full, s_q + w * Shape::kTileBytes + x * kBlockBytes, x * 64, u.head0,
+                          u.row0 + w * p.tpt);
+        }
+        ++q_loads;
+        auto page_of = [&](int32_t i) -> int32_t {
+          const int32_t j0 = tiles.tile(i) * kTile + sub * box_rows;
+          const bool seen = j0 <= last && (j0 + box_rows > low || j0 < a.sinks);
+          if (!seen) return static_cast<int32_t>(c.num_pages);
+          const int32_t id = __ldg(c.table + u.b * c.table_stride + (j0 >> c.page_shift));
+          if (id >= 0 && id < c.num_pages) return id;
+          raise_bad_arg(c.err);
+          return static_cast<int32_t>(c.num_pages);
+        };
+        int32_t page = page_of(0);
+        for (int32_t i = 0; i < tiles.n && ok; ++i) {
+          const int32_t next = i + 1 < tiles.n ? page_of(i + 1) : 0;
+          const int32_t j0 = tiles.tile(i) * kTile;
+          const bool whole = j0 + kTile <= last + 1 && (j0 >= low || j0 + kTile <= a.sinks);
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {
+            if (!(ok = warp_wait(kv_empty + stage, phase ^ 1u, abort_flag, c.err))) break;
+            uint64_t* bar = (v == 1 && !whole ? landed : kv_full) + stage;
+            if (lane == 0) mbar_arrive_expect_tx(bar, Shape::kTileBytes);
+            __syncwarp();
+            if (lane < boxes)
+              tma_load_4d(v == 1 ? &tm_v : &tm_k, bar,
+                          s_kv + stage * Shape::kTileBytes + block * kBlockBytes + sub * box_rows * 128, block * 64,
+                          (j0 + sub * box_rows) & (page_size - 1), u.kvh, page);
+            ++issued;
+            if (v == 1 && !whole) {
+              by_landed |= 1u << stage;
+              land_parity ^= 1u << stage;
+            } else {
+              by_landed &= ~(1u << stage);
+            }
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
+          }
+          page = next;
+        }
+      }
+      if (!ok || *abort_flag) {
+        // let the copies in flight land before the CTA exits
+        volatile uint32_t no_abort = 0;
+        if (q_loads > 0) mbar_wait(q_full, static_cast<uint32_t>((q_loads - 1) & 1), &no_abort, c.err);
+        // (all but a stage's last tile have been used, so they are complete)
+        for (int s = 0; s < kStages && s < issued; ++s) {
+          const uint32_t uses = (issued - s + kStages - 1) / kStages;
+          if ((by_landed >> s) & 1u) mbar_wait(landed + s, ((land_parity >> s) & 1u) ^ 1u, &no_abort, c.err);
+          else mbar_wait(kv_full + s, (uses - 1) & 1u, &no_abort, c.err);
+        }
+      }
+    } else if (warp == 10) {
+      // ------------------------------------------------------------------ zeroing of unseen V rows
+      uint32_t stage = 0, land_phase = 0;  // one parity bit per stage
+      bool ok = true;
+      Unit u;
+      while (ok && next_unit(u)) {
+        const TileList<kTile> tiles = tiles_of(u);
+        const int32_t last = u.pos0 + u.count - 1;
+        const int32_t low = a.window > 0 && u.pos0 >= a.window ? u.pos0 - a.window + 1 : 0;
+        for (int32_t i = 0; i < tiles.n; ++i) {
+          const int32_t j0 = tiles.tile(i) * kTile;
+          const bool whole = j0 + kTile <= last + 1 && (j0 >= low || j0 + kTile <= a.sinks);
+          if (++stage >= kStages) stage -= kStages;  // past the K tile
+          if (!whole) {
+            if (!(ok = warp_wait(landed + stage, (land_phase >> stage) & 1u, abort_flag, c.err))) break;
+            land_phase ^= 1u << stage;
+            uint8_t* v = s_kv + stage * Shape::kTileBytes;
+            // lanes 8 x .. 8 x + 7 write the eight 16-byte parts of row x (of four at a time)
+            for (int r = lane >> 3; r < kTile; r += 4) {
+              const int32_t j = j0 + r;
+              if (j <= last && (j >= low || j < a.sinks)) continue;
+#pragma unroll
+              for (int x = 0; x < kBlocks; ++x)
+                *reinterpret_cast<uint4*>(v + x * kBlockBytes + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(kv_full + stage);
+          }
+          if (++stage >= kStages) stage -= kStages;
+        }
+      }
+    } else {
+      // ------------------------------------------------------------------ products (one lane)
+      constexpr uint32_t idesc_s = BF16 ? idesc_bf16(128, kTile) : idesc_f16(128, kTile);
+      constexpr uint32_t idesc_o = (BF16 ? idesc_bf16(128, D) : idesc_f16(128, D)) | (1u << 16);  // V MN-major
+      uint32_t q_phase = 0, p_phase[2] = {0, 0};
+      uint32_t ring = 0;  // K and V tiles before this unit
+      bool ok = true, any = false;
+      Unit u;
+      while (ok && next_unit(u)) {
+        const TileList<kTile> tiles = tiles_of(u);
+        if (tiles.n == 0) continue;
+        if (lane == 0) {
+          const TileRows rows[2] = {TileRows(p, u, 0), TileRows(p, u, 1)};
+          auto meets = [&](int w, int32_t i) { return rows[w].meets(tiles.tile(i), a.sinks); };
+          auto next_of = [&](int w, int32_t i) {
+            while (++i < tiles.n && !meets(w, i)) {
+            }
+            return i;
+          };
+          auto full = [&](uint32_t at) { return mbar_wait(kv_full + at % kStages, (at / kStages) & 1u, abort_flag, c.err); };
+          auto scores = [&](int w, int32_t i) -> bool {
+            const uint32_t at = ring + 2 * i;
+            if (!full(at)) return false;
+            tc_fence_after();
+            const uint32_t qa = smem_u32(s_q + w * Shape::kTileBytes);
+            const uint32_t ka = smem_u32(s_kv + (at % kStages) * Shape::kTileBytes);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t off = (k >> 2) * kBlockBytes + (k & 3) * 32;
+              mma_f16(tmem + Shape::kColS + w * kTile, smem_desc_sw128_kmajor(qa + off), smem_desc_sw128_kmajor(ka + off),
+                      idesc_s, k != 0 ? 1u : 0u);
+            }
+            mma_commit(s_full + w);
+            mma_commit(kv_empty + at % kStages);
+            any = true;
+            return true;
+          };
+          ok = mbar_wait(q_full, q_phase, abort_flag, c.err);
+          q_phase ^= 1u;
+          int open = 0;  // row tiles that still have scores to come
+          int32_t done[2] = {0, 0};
+          for (int w = 0; w < 2 && ok; ++w) {
+            const int32_t i = next_of(w, -1);
+            if (i < tiles.n) {
+              ok = scores(w, i);
+              if (next_of(w, i) < tiles.n) ++open;
+            }
+          }
+          if (ok && open == 0) mma_commit(q_empty);
+          for (int32_t i = 0; i < tiles.n && ok; ++i) {
+            const uint32_t at = ring + 2 * i + 1;
+            for (int w = 0; w < 2 && ok; ++w) {
+              if (!meets(w, i)) {
+                mbar_arrive(kv_empty + (at - 1) % kStages);
+                mbar_arrive(kv_empty + at % kStages);
+                continue;
+              }
+              if (!(ok = mbar_wait(p_full + w, p_phase[w], abort_flag, c.err))) break;
+              p_phase[w] ^= 1u;
+              if (!(ok = full(at))) break;
+              tc_fence_after();
+              const uint32_t va = smem_u32(s_kv + (at % kStages) * Shape::kTileBytes);
+#pragma unroll
+              for (int k = 0; k < kTile / 16; ++k)
+                mma_f16_ts(tmem + Shape::kColO + w * D, tmem + Shape::kColS + w * kTile + k * 8,
+                           smem_desc_sw128_mnmajor(va + k * 2048, kBlockBytes), idesc_o, (done[w] | k) != 0 ? 1u : 0u);
+              done[w] = 1;
+              mma_commit(kv_empty + at % kStages);
+              const int32_t j = next_of(w, i);
+              if (j < tiles.n) {
+                if (!(ok = scores(w, j))) break;
+                if (next_of(w, j) >= tiles.n && --open == 0) mma_commit(q_empty);
+              } else {
+                mma_commit(o_full + w);
+              }
+            }
+          }
+          ring += 2 * tiles.n;
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+      }
+      if (lane == 0 && any && (!ok || *abort_flag)) {
+        volatile uint32_t no_abort = 0;
+        mma_commit(drain);
+        mbar_wait(drain, 0u, &no_abort, c.err);
+      }
+      __syncwarp();
+    }
+  } else {
+    // -------------------------------------------------------------------- softmax and output
+    regs_grow<208>();
+    const int w = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t t_s = tmem + lanes + Shape::kColS + w * kTile;
+    const uint32_t t_o = tmem + lanes + Shape::kColO + w * D;
+    const int token = row / p.hp, head = row - token * p.hp;
+    const float scale = a.scale_log2;
+    uint32_t s_phase = 0, o_phase = 0;
+    Unit u;
+    bool ok = true;
+    while (ok && next_unit(u)) {
+      const TileList<kTile> tiles = tiles_of(u);
+      const TileRows rows(p, u, w);
+      if (rows.count == 0) continue;
+      const bool mine = token < rows.count;
+      // positions of this row and of the warp's first and last one
+      const int32_t pos = rows.first + (mine ? token : rows.count - 1);
+      const int32_t low = a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;
+      const int32_t pos_min = __shfl_sync(0xffffffffu, pos, 0), low_max = __shfl_sync(0xffffffffu, low, 31);
+      float ref = -INFINITY;  // the reference m, in units of the raw scores
+      float l = 0.0f;
+      int done = 0;
+      for (int32_t i = 0; i < tiles.n; ++i) {
+        const int32_t j0 = tiles.tile(i) * kTile;
+        if (!rows.meets(tiles.tile(i), a.sinks)) continue;
+        if (!(ok = warp_wait(s_full + w, s_phase, abort_flag, c.err))) break;
+        s_phase ^= 1u;
+        tc_fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmem_ld_32x32b_x32(t_s + 32 * x, s[x]);
+        tmem_ld_wait();
+        if (j0 + kTile - 1 > pos_min || (j0 < low_max && j0 + kTile > a.sinks)) {
+          // some row of the warp does not see the whole tile
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (!key_visible(j0 + 32 * x + e, pos, low, a.sinks)) s[x][e] = 0xFF800000u;
+        }
+        float top[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          top[x] = __uint_as_float(s[x][0]);
+#pragma unroll
+          for (int e = 1; e < 32; ++e) top[x] = fmaxf(top[x], __uint_as_float(s[x][e]));
+        }
+        const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        if (done == 0) {
+          ref = m;
+        } else {
+          // also true where ref is -inf and m is not; false where both are
+          const bool move = (m - ref) * scale > kMoveBy;
+          if (__any_sync(0xffffffffu, move)) {
+            const float f = move ? ex2_approx((ref - m) * scale) : 1.0f;
+            if (move) ref = m;
+            l *= f;
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(t_o + 32 * x, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st_32x32b_x32(t_o + 32 * x, o);
+            }
+          }
+        }
+        done = 1;
+        const float shift = ref == -INFINITY ? 0.0f : -ref * scale;
+        const uint64_t scale2 = f2pack(scale, scale), shift2 = f2pack(shift, shift);
+        uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float y0, y1;
+            f2unpack(f2fma(f2pack(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), scale2, shift2), y0, y1);
+            y0 = ex2_approx(y0);
+            y1 = ex2_approx(y1);
+            sum2[e & 1] = f2add(sum2[e & 1], f2pack(y0, y1));
+            packed[e] = pack16<BF16>(y0, y1);
+          }
+          tmem_st_32x32b_x16(t_s + 16 * x, packed);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + w);
+        float s0, s1;
+        f2unpack(f2add(sum2[0], sum2[1]), s0, s1);
+        l += s0 + s1;
+      }
+      if (!ok) break;
+      if (done) {
+        if (!(ok = warp_wait(o_full + w, o_phase, abort_flag, c.err))) break;
+        o_phase ^= 1u;
+        tc_fence_after();
+      }
+      const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
+      const int64_t at = (static_cast<int64_t>(u.row0 + w * p.tpt + token) * a.q_heads + u.head0 + head) * D;
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) {
+        uint32_t o[32];
+        if (done) {
+          tmem_ld_32x32b_x32(t_o + 32 * x, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0u;
+        }
+        __syncwarp();
+        if (mine) {
+        float y[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * inv;
+        if (a.out) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            *reinterpret_cast<uint4*>(a.out + at + 32 * x + 8 * v) =
+                make_uint4(pack16<BF16>(y[8 * v], y[8 * v + 1]), pack16<BF16>(y[8 * v + 2], y[8 * v + 3]),
+                           pack16<BF16>(y[8 * v + 4], y[8 * v + 5]), pack16<BF16>(y[8 * v + 6], y[8 * v + 7]));
+        }
+        if (a.out_i8) {
+          uint32_t pk[8];
+          requant_pack<32>(y, a.s_out, a.inv_s_out, false, a.rounding, pk);
+#pragma unroll
+          for (int v = 0; v < 2; ++v)
+            *reinterpret_cast<uint4*>(a.out_i8 + at + 32 * x + 16 * v) =
+                make_uint4(pk[4 * v], pk[4 * v + 1], pk[4 * v + 2], pk[4 * v + 3]);
+        }
+        }
+        __syncwarp();
+      }
+      // the next unit's products into O follow p_full, which this warp signals behind these loads
+      tc_fence_before();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <bool BF16, int D>
+lsc_status launch_prefill(const lsc_paged_kv* cache, const DeviceState* ds, const PagedView& c, PrefillArgs p,
+                          cudaStream_t st) {
+  using Shape = PrefillShape<D>;
+  const AttnArgs& a = p.a;
+  const uint32_t box = cache->page_size < kTile ? cache->page_size : kTile;
+  CUtensorMap tq, tk, tv;
+  lsc_status s = paged_tensor_map(&tk, cache, c, cache->k, box);
+  if (s == LSC_SUCCESS) s = paged_tensor_map(&tv, cache, c, cache->v, box);
+  if (s) return s;
+  const uint64_t dims[3] = {D, static_cast<uint64_t>(a.q_heads), static_cast<uint64_t>(a.tokens)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(a.q_head) * 2, static_cast<uint64_t>(a.q_token) * 2};
+  const uint32_t qbox[3] = {64, static_cast<uint32_t>(p.hp), static_cast<uint32_t>(p.tpt)};
+  const uint32_t ones[3] = {1, 1, 1};
+  s = encode_tmap_3d(&tq, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.q, dims, strides,
+                     qbox, ones, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (s) return s;
+  // units: at most one short one per sequence beside the full ones
+  auto units = [&](int64_t tokens) {
+    return (a.tokens / tokens + (a.tokens < c.batch ? a.tokens : c.batch)) * p.pairs;
+  };
+  // two row tiles per unit hide one's softmax behind the other's products; with fewer units than SMs
+  // one row tile each spreads the work over more of them
+  p.unit_tokens = units(2 * p.tpt) < ds->sm_count ? p.tpt : 2 * p.tpt;
+  const int64_t most = units(p.unit_tokens);
+  const int grid = static_cast<int>(most < ds->sm_count ? most : ds->sm_count);
+  LSC_CUDA_TRY(cudaFuncSetAttribute(paged_prefill_kernel<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    Shape::kSmem));
+  LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, paged_prefill_kernel<BF16, D>, dim3(grid), dim3(kPrefillThreads),
+                                Shape::kSmem, st, tq, tk, tv, c, p));
+  return LSC_SUCCESS;
+}
+
+}  // namespace
+
+lsc_status attention_args(const lsc_paged_kv* cache, const char* who, const void* q, int64_t tokens, int32_t q_heads,
+                          int64_t q_token, int64_t q_head, float alpha, int64_t window, int64_t sinks, void* out,
+                          int8_t* out_i8, float s_out, int32_t rounding, AttnArgs* a) {
+  if (tokens < 0 || tokens > INT32_MAX) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: bad token count", who);
+  if (q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads)
+    return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: %d query heads are not a multiple of %d key-value heads", who,
+                     q_heads, cache->kv_heads);
+  if (!(alpha > 0.0f) || !(alpha <= 1.0e38f))
+    return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: alpha must be positive and finite", who);
+  if (window < 0 || sinks < 0) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: negative window or sinks", who);
+  if (rounding != LSC_ROUND_HALF_AWAY && rounding != LSC_ROUND_HALF_EVEN)
+    return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: bad rounding %d", who, rounding);
+  // the stride of an axis of one entry is never used: any value will do there
+  if (q_heads == 1) q_head = cache->head_dim;
+  if (tokens <= 1) q_token = static_cast<int64_t>(q_heads) * cache->head_dim;
+  if (q_token < 0 || q_head < 0 || q_token % 8 || q_head % 8 || q_token >= (int64_t{1} << 39) ||
+      q_head >= (int64_t{1} << 39))
+    return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: query strides must be multiples of 8 elements", who);
+  if (tokens > 0 && cache->batch > 0) {
+    if (!q || (!out && !out_i8)) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: null pointer", who);
+    if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_i8)) & 15)
+      return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", who);
+    if (out_i8 && !(s_out > 0.0f))
+      return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: int8 output needs a scale > 0", who);
+  }
+  a->q = static_cast<const uint16_t*>(q);
+  a->tokens = tokens;
+  a->q_token = q_token;
+  a->q_head = q_head;
+  a->q_heads = q_heads;
+  a->group = q_heads / cache->kv_heads;
+  a->scale_log2 = alpha * kLog2e;
+  // positions stay below 2^30: a longer window is no window, more sinks see no more
+  a->window = static_cast<int32_t>(window > (1 << 30) ? 0 : window);
+  a->sinks = static_cast<int32_t>(window == 0 ? 0 : (sinks > (1 << 30) ? (1 << 30) : sinks));
+  a->out = static_cast<uint16_t*>(out);
+  a->out_i8 = out_i8;
+  a->s_out = s_out;
+  a->inv_s_out = out_i8 ? reciprocal_or_zero(s_out) : 0.0f;
+  a->rounding = rounding;
+  a->offsets = nullptr;
+  return LSC_SUCCESS;
+}
+
+lsc_status paged_tensor_map(CUtensorMap* map, const lsc_paged_kv* cache, const PagedView& view, const void* base,
+                            uint32_t box_rows) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(cache->head_dim), static_cast<uint64_t>(cache->page_size),
+                            static_cast<uint64_t>(cache->kv_heads), static_cast<uint64_t>(cache->num_pages)};
+  const uint64_t strides[3] = {static_cast<uint64_t>(view.token_stride) * 2, static_cast<uint64_t>(view.head_stride) * 2,
+                               static_cast<uint64_t>(view.page_stride) * 2};
+  const uint32_t box[4] = {64, box_rows, 1, 1};
+  const uint32_t ones[4] = {1, 1, 1, 1};
+  return encode_tmap_4d(map, cache->dtype == LSC_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        base, dims, strides, box, ones, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+}  // namespace lsc
+
+using namespace lsc;
+
+extern "C" lsc_status lsc_paged_attention_prefill(const lsc_paged_kv* cache, const void* q, int64_t tokens,
+                                                  int32_t q_heads, int64_t q_token_stride, int64_t q_head_stride,
+                                                  const int32_t* q_offsets, float alpha, int64_t window, int64_t sinks,
+                                                  void* out, int8_t* out_i8, float s_out, int32_t rounding,
+                                                  lsc_stream stream) {
+  const char* who = "paged_attention_prefill";
+  PagedView c;
+  PrefillArgs p{};
+  lsc_status st = paged_view(cache, who, &c);
+  if (st) return st;
+  st = attention_args(cache, who, q, tokens, q_heads, q_token_stride, q_head_stride, alpha, window, sinks, out, out_i8,
+                      s_out, rounding, &p.a);
+  if (st) return st;
+  if (tokens == 0 || c.batch == 0) return LSC_SUCCESS;
+  if (!q_offsets) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: null offsets", who);
+  p.a.offsets = q_offsets;
+  DeviceState* ds = nullptr;
+  if ((st = paged_device(who, &ds, &c))) return st;
+  // heads of a row tile: the group, or its largest divisor up to 32
+  p.hp = p.a.group;
+  if (p.hp > 32)
+    for (p.hp = 32; p.a.group % p.hp; --p.hp) {
+    }
+  p.tpt = kTile / p.hp;
+  p.pairs = c.kv_heads * (p.a.group / p.hp);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf16 = cache->dtype == LSC_DTYPE_BF16;
+  if (cache->head_dim == 64)
+    return bf16 ? launch_prefill<true, 64>(cache, ds, c, p, s) : launch_prefill<false, 64>(cache, ds, c, p, s);
+  return bf16 ? launch_prefill<true, 128>(cache, ds, c, p, s) : launch_prefill<false, 128>(cache, ds, c, p, s);
+}
