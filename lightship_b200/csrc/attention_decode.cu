@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
           float x = s[n][e] * a.scale_log2;
           if (edge) {
             const int32_t j = t0 + n * 8 + cpair + (e & 1);
-            if (!(j < cur.len && (j >= low || j < a.sinks))) x = -INFINITY;
+            x = key_visible(j, cur.len - 1, low, a.sinks) ? x : -INFINITY;
           }
           s[n][e] = x;
           top[e >> 1] = fmaxf(top[e >> 1], x);
@@ -397,7 +397,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
         uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
         if (edge) {
           const int32_t j = t0 + n * 16 + cpair;
-          auto keep = [&](int32_t x) { return x < cur.len && (x >= low || x < a.sinks); };
+          auto keep = [&](int32_t x) { return key_visible(x, cur.len - 1, low, a.sinks); };
           keep0 = (keep(j) ? 0xFFFFu : 0u) | (keep(j + 1) ? 0xFFFF0000u : 0u);
           keep1 = (keep(j + 8) ? 0xFFFFu : 0u) | (keep(j + 9) ? 0xFFFF0000u : 0u);
         }

@@ -73,6 +73,32 @@ struct TileRows {
   }
 };
 
+// The numbers (in a unit's tile list) of the tiles that a row tile meets: the first `kept` and
+// [from, to).
+struct TileSpan {
+  int32_t kept, from, to, n;
+  __device__ __forceinline__ TileSpan(const TileRows& r, const TileList<kTile>& tiles, int32_t sinks) {
+    n = tiles.n;
+    const int32_t shift = tiles.sink_tiles - tiles.start;  // key tile -> number, behind the sinks' tiles
+    to = r.count > 0 && r.last >= 0 ? r.last / kTile + 1 + shift : 0;
+    from = r.low / kTile + shift;
+    from = from < tiles.sink_tiles ? tiles.sink_tiles : from;
+    // with the sinks' tiles in front of the list, all tiles up to the one before the window's first
+    // that hold a sink
+    const int32_t sink_tiles = sinks > 0 ? (sinks - 1) / kTile + 1 : 0;
+    kept = tiles.sink_tiles > 0 ? tiles.sink_tiles : sink_tiles;
+    kept = kept < to ? kept : to;
+    if (kept >= from) kept = from = 0;
+  }
+  __device__ __forceinline__ bool has(int32_t i) const { return i < kept || (i >= from && i < to); }
+  // the number after i (n: none)
+  __device__ __forceinline__ int32_t next(int32_t i) const {
+    ++i;
+    if (i >= kept && i < from) i = from;
+    return i < to ? i : n;
+  }
+};
+
 // The units of this CTA, found by one warp.  Sequence b's units stand at levels
 // base_b .. base_b + n_b - 1 (its position in units); F(t) counts those at level t or above.
 struct Scheduler {
@@ -384,82 +410,93 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       }
     } else {
       // ------------------------------------------------------------------ products (one lane)
+      // The thread that issues shares its scheduler with softmax warps, so the loop keeps few
+      // instructions: descriptors are a 64-bit base plus constants, tile numbers are ranges.
       constexpr uint32_t idesc_s = BF16 ? idesc_bf16(128, kTile) : idesc_f16(128, kTile);
       constexpr uint32_t idesc_o = (BF16 ? idesc_bf16(128, D) : idesc_f16(128, D)) | (1u << 16);  // V MN-major
+      const uint64_t dq[2] = {smem_desc_sw128_kmajor(smem_u32(s_q)),
+                              smem_desc_sw128_kmajor(smem_u32(s_q + Shape::kTileBytes))};
+      const uint64_t dk = smem_desc_sw128_kmajor(smem_u32(s_kv));
+      const uint64_t dv = smem_desc_sw128_mnmajor(smem_u32(s_kv), kBlockBytes);
       uint32_t q_phase = 0, p_phase[2] = {0, 0};
-      uint32_t ring = 0;  // K and V tiles before this unit
+      uint32_t stage0 = 0, phase0 = 0;  // of the unit's first K tile
       bool ok = true, any = false;
       Unit u;
       while (ok && next_unit(u)) {
         const TileList<kTile> tiles = tiles_of(u);
         if (tiles.n == 0) continue;
         if (lane == 0) {
-          const TileRows rows[2] = {TileRows(p, u, 0), TileRows(p, u, 1)};
-          auto meets = [&](int w, int32_t i) { return rows[w].meets(tiles.tile(i), a.sinks); };
-          auto next_of = [&](int w, int32_t i) {
-            while (++i < tiles.n && !meets(w, i)) {
-            }
-            return i;
+          const TileSpan span[2] = {TileSpan(TileRows(p, u, 0), tiles, a.sinks), TileSpan(TileRows(p, u, 1), tiles, a.sinks)};
+          // stage and phase of tile `x` (K tiles even, V tiles odd) of the unit
+          auto at = [&](int32_t x, uint32_t& stage, uint32_t& phase) {
+            const uint32_t y = stage0 + static_cast<uint32_t>(x);
+            stage = y % kStages;
+            phase = phase0 ^ ((y / kStages) & 1u);
           };
-          auto full = [&](uint32_t at) { return mbar_wait(kv_full + at % kStages, (at / kStages) & 1u, abort_flag, c.err); };
           auto scores = [&](int w, int32_t i) -> bool {
-            const uint32_t at = ring + 2 * i;
-            if (!full(at)) return false;
+            uint32_t stage, phase;
+            at(2 * i, stage, phase);
+            if (!mbar_wait(kv_full + stage, phase, abort_flag, c.err)) return false;
             tc_fence_after();
-            const uint32_t qa = smem_u32(s_q + w * Shape::kTileBytes);
-            const uint32_t ka = smem_u32(s_kv + (at % kStages) * Shape::kTileBytes);
+            const uint64_t dka = dk + stage * (Shape::kTileBytes >> 4);
+            const uint64_t dqa = w ? dq[1] : dq[0];
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-              const uint32_t off = (k >> 2) * kBlockBytes + (k & 3) * 32;
-              mma_f16(tmem + Shape::kColS + w * kTile, smem_desc_sw128_kmajor(qa + off), smem_desc_sw128_kmajor(ka + off),
-                      idesc_s, k != 0 ? 1u : 0u);
+              constexpr int kStep = 32 >> 4, kBlock = kBlockBytes >> 4;
+              mma_f16(tmem + Shape::kColS + w * kTile, dqa + (k >> 2) * kBlock + (k & 3) * kStep,
+                      dka + (k >> 2) * kBlock + (k & 3) * kStep, idesc_s, k != 0 ? 1u : 0u);
             }
             mma_commit(s_full + w);
-            mma_commit(kv_empty + at % kStages);
+            mma_commit(kv_empty + stage);
             any = true;
             return true;
           };
           ok = mbar_wait(q_full, q_phase, abort_flag, c.err);
           q_phase ^= 1u;
           int open = 0;  // row tiles that still have scores to come
-          int32_t done[2] = {0, 0};
+          uint32_t more[2] = {0, 0};
           for (int w = 0; w < 2 && ok; ++w) {
-            const int32_t i = next_of(w, -1);
+            const int32_t i = span[w].next(-1);
             if (i < tiles.n) {
               ok = scores(w, i);
-              if (next_of(w, i) < tiles.n) ++open;
+              if (span[w].next(i) < tiles.n) ++open;
             }
           }
           if (ok && open == 0) mma_commit(q_empty);
           for (int32_t i = 0; i < tiles.n && ok; ++i) {
-            const uint32_t at = ring + 2 * i + 1;
-            for (int w = 0; w < 2 && ok; ++w) {
-              if (!meets(w, i)) {
-                mbar_arrive(kv_empty + (at - 1) % kStages);
-                mbar_arrive(kv_empty + at % kStages);
+            uint32_t stage, phase;
+            at(2 * i + 1, stage, phase);
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              if (!ok) break;
+              if (!span[w].has(i)) {
+                mbar_arrive(kv_empty + (stage == 0 ? kStages - 1 : stage - 1));
+                mbar_arrive(kv_empty + stage);
                 continue;
               }
               if (!(ok = mbar_wait(p_full + w, p_phase[w], abort_flag, c.err))) break;
               p_phase[w] ^= 1u;
-              if (!(ok = full(at))) break;
+              if (!(ok = mbar_wait(kv_full + stage, phase, abort_flag, c.err))) break;
               tc_fence_after();
-              const uint32_t va = smem_u32(s_kv + (at % kStages) * Shape::kTileBytes);
+              const uint64_t dva = dv + stage * (Shape::kTileBytes >> 4);
 #pragma unroll
               for (int k = 0; k < kTile / 16; ++k)
-                mma_f16_ts(tmem + Shape::kColO + w * D, tmem + Shape::kColS + w * kTile + k * 8,
-                           smem_desc_sw128_mnmajor(va + k * 2048, kBlockBytes), idesc_o, (done[w] | k) != 0 ? 1u : 0u);
-              done[w] = 1;
-              mma_commit(kv_empty + at % kStages);
-              const int32_t j = next_of(w, i);
+                mma_f16_ts(tmem + Shape::kColO + w * D, tmem + Shape::kColS + w * kTile + k * 8, dva + k * (2048 >> 4),
+                           idesc_o, k != 0 ? 1u : more[w]);
+              more[w] = 1;
+              mma_commit(kv_empty + stage);
+              const int32_t j = span[w].next(i);
               if (j < tiles.n) {
                 if (!(ok = scores(w, j))) break;
-                if (next_of(w, j) >= tiles.n && --open == 0) mma_commit(q_empty);
+                if (span[w].next(j) >= tiles.n && --open == 0) mma_commit(q_empty);
               } else {
                 mma_commit(o_full + w);
               }
             }
           }
-          ring += 2 * tiles.n;
+          const uint32_t y = stage0 + 2u * static_cast<uint32_t>(tiles.n);
+          phase0 ^= (y / kStages) & 1u;
+          stage0 = y % kStages;
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
@@ -508,10 +545,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         if (j0 + kTile - 1 > pos_min || (j0 < low_max && j0 + kTile > a.sinks)) {
           // some row of the warp does not see the whole tile
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t see = visible_mask(j0 + 32 * x, pos, low, a.sinks);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!key_visible(j0 + 32 * x + e, pos, low, a.sinks)) s[x][e] = 0xFF800000u;
+            for (int e = 0; e < 32; ++e) s[x][e] = (see >> e) & 1u ? s[x][e] : 0xFF800000u;
+          }
         }
         float top[4];
 #pragma unroll

@@ -57,7 +57,17 @@ __device__ __forceinline__ void check_rows(const PagedView& c, const int32_t* __
 
 // Key j as the query at position p sees it.  `low` = p - window + 1, or 0 without a window.
 __device__ __forceinline__ bool key_visible(int32_t j, int32_t p, int32_t low, int32_t sinks) {
-  return j <= p && (j >= low || j < sinks);
+  return (j <= p) & ((j >= low) | (j < sinks));
+}
+
+// Bits 0 .. n - 1 (all for n >= 32, none for n <= 0).
+__device__ __forceinline__ uint32_t low_bits(int32_t n) {
+  return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << n) - 1u);
+}
+
+// key_visible of keys j .. j + 31, as bits.
+__device__ __forceinline__ uint32_t visible_mask(int32_t j, int32_t p, int32_t low, int32_t sinks) {
+  return low_bits(p - j + 1) & (~low_bits(low - j) | low_bits(sinks - j));
 }
 
 }  // namespace lsc
