@@ -409,13 +409,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         }
       }
     } else {
-      // ------------------------------------------------------------------ products (one lane)
-      // The thread that issues shares its scheduler with softmax warps, so the loop keeps few
-      // instructions: descriptors are a 64-bit base plus constants, tile numbers are ranges.
+      // ------------------------------------------------------------------ products
+      // The whole warp walks the tiles and one elected lane issues: a lane that has left its warp
+      // issues at half the rate.  Descriptors are a 64-bit base plus constants.
       constexpr uint32_t idesc_s = BF16 ? idesc_bf16(128, kTile) : idesc_f16(128, kTile);
       constexpr uint32_t idesc_o = (BF16 ? idesc_bf16(128, D) : idesc_f16(128, D)) | (1u << 16);  // V MN-major
-      const uint64_t dq[2] = {smem_desc_sw128_kmajor(smem_u32(s_q)),
-                              smem_desc_sw128_kmajor(smem_u32(s_q + Shape::kTileBytes))};
+      const uint64_t dq = smem_desc_sw128_kmajor(smem_u32(s_q));
       const uint64_t dk = smem_desc_sw128_kmajor(smem_u32(s_kv));
       const uint64_t dv = smem_desc_sw128_mnmajor(smem_u32(s_kv), kBlockBytes);
       uint32_t q_phase = 0, p_phase[2] = {0, 0};
@@ -425,21 +424,22 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       while (ok && next_unit(u)) {
         const TileList<kTile> tiles = tiles_of(u);
         if (tiles.n == 0) continue;
-        if (lane == 0) {
-          const TileSpan span[2] = {TileSpan(TileRows(p, u, 0), tiles, a.sinks), TileSpan(TileRows(p, u, 1), tiles, a.sinks)};
-          // stage and phase of tile `x` (K tiles even, V tiles odd) of the unit
-          auto at = [&](int32_t x, uint32_t& stage, uint32_t& phase) {
-            const uint32_t y = stage0 + static_cast<uint32_t>(x);
-            stage = y % kStages;
-            phase = phase0 ^ ((y / kStages) & 1u);
-          };
-          auto scores = [&](int w, int32_t i) -> bool {
-            uint32_t stage, phase;
-            at(2 * i, stage, phase);
-            if (!mbar_wait(kv_full + stage, phase, abort_flag, c.err)) return false;
-            tc_fence_after();
-            const uint64_t dka = dk + stage * (Shape::kTileBytes >> 4);
-            const uint64_t dqa = w ? dq[1] : dq[0];
+        const TileSpan span[2] = {TileSpan(TileRows(p, u, 0), tiles, a.sinks), TileSpan(TileRows(p, u, 1), tiles, a.sinks)};
+        // stage and phase of tile `x` (K tiles even, V tiles odd) of the unit
+        auto at = [&](int32_t x, uint32_t& stage, uint32_t& phase) {
+          const uint32_t y = stage0 + static_cast<uint32_t>(x);
+          stage = y % kStages;
+          phase = phase0 ^ ((y / kStages) & 1u);
+        };
+        // S of row tile w and tile i; `last`: Q is not needed after it
+        auto scores = [&](int w, int32_t i, bool last) -> bool {
+          uint32_t stage, phase;
+          at(2 * i, stage, phase);
+          if (!warp_wait(kv_full + stage, phase, abort_flag, c.err)) return false;
+          tc_fence_after();
+          const uint64_t dka = dk + stage * (Shape::kTileBytes >> 4);
+          const uint64_t dqa = dq + w * (Shape::kTileBytes >> 4);
+          if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
               constexpr int kStep = 32 >> 4, kBlock = kBlockBytes >> 4;
@@ -448,64 +448,71 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             }
             mma_commit(s_full + w);
             mma_commit(kv_empty + stage);
-            any = true;
-            return true;
-          };
-          ok = mbar_wait(q_full, q_phase, abort_flag, c.err);
-          q_phase ^= 1u;
-          int open = 0;  // row tiles that still have scores to come
-          uint32_t more[2] = {0, 0};
-          for (int w = 0; w < 2 && ok; ++w) {
-            const int32_t i = span[w].next(-1);
-            if (i < tiles.n) {
-              ok = scores(w, i);
-              if (span[w].next(i) < tiles.n) ++open;
-            }
+            if (last) mma_commit(q_empty);
           }
-          if (ok && open == 0) mma_commit(q_empty);
-          for (int32_t i = 0; i < tiles.n && ok; ++i) {
-            uint32_t stage, phase;
-            at(2 * i + 1, stage, phase);
+          __syncwarp();
+          any = true;
+          return true;
+        };
+        if (!(ok = warp_wait(q_full, q_phase, abort_flag, c.err))) break;
+        q_phase ^= 1u;
+        int open = 0;  // row tiles that still have scores to come
+        uint32_t more[2] = {0, 0};
+        const int32_t first[2] = {span[0].next(-1), span[1].next(-1)};
 #pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              if (!ok) break;
-              if (!span[w].has(i)) {
+        for (int w = 0; w < 2; ++w)
+          if (first[w] < tiles.n && span[w].next(first[w]) < tiles.n) ++open;
+        if (first[0] < tiles.n) ok = scores(0, first[0], open == 0 && first[1] >= tiles.n);
+        if (ok && first[1] < tiles.n) ok = scores(1, first[1], open == 0);
+        for (int32_t i = 0; i < tiles.n && ok; ++i) {
+          uint32_t stage, phase;
+          at(2 * i + 1, stage, phase);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (!ok) break;
+            if (!span[w].has(i)) {
+              if (lane == 0) {
                 mbar_arrive(kv_empty + (stage == 0 ? kStages - 1 : stage - 1));
                 mbar_arrive(kv_empty + stage);
-                continue;
               }
-              if (!(ok = mbar_wait(p_full + w, p_phase[w], abort_flag, c.err))) break;
-              p_phase[w] ^= 1u;
-              if (!(ok = mbar_wait(kv_full + stage, phase, abort_flag, c.err))) break;
-              tc_fence_after();
-              const uint64_t dva = dv + stage * (Shape::kTileBytes >> 4);
+              __syncwarp();
+              continue;
+            }
+            if (!(ok = warp_wait(p_full + w, p_phase[w], abort_flag, c.err))) break;
+            p_phase[w] ^= 1u;
+            if (!(ok = warp_wait(kv_full + stage, phase, abort_flag, c.err))) break;
+            tc_fence_after();
+            const uint64_t dva = dv + stage * (Shape::kTileBytes >> 4);
+            const int32_t j = span[w].next(i);
+            if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < kTile / 16; ++k)
                 mma_f16_ts(tmem + Shape::kColO + w * D, tmem + Shape::kColS + w * kTile + k * 8, dva + k * (2048 >> 4),
                            idesc_o, k != 0 ? 1u : more[w]);
-              more[w] = 1;
               mma_commit(kv_empty + stage);
-              const int32_t j = span[w].next(i);
-              if (j < tiles.n) {
-                if (!(ok = scores(w, j))) break;
-                if (span[w].next(j) >= tiles.n && --open == 0) mma_commit(q_empty);
-              } else {
-                mma_commit(o_full + w);
-              }
+              if (j >= tiles.n) mma_commit(o_full + w);
+            }
+            __syncwarp();
+            more[w] = 1;
+            if (j < tiles.n) {
+              const bool end = span[w].next(j) >= tiles.n;
+              if (end) --open;
+              ok = scores(w, j, end && open == 0);
             }
           }
-          const uint32_t y = stage0 + 2u * static_cast<uint32_t>(tiles.n);
-          phase0 ^= (y / kStages) & 1u;
-          stage0 = y % kStages;
         }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        const uint32_t y = stage0 + 2u * static_cast<uint32_t>(tiles.n);
+        phase0 ^= (y / kStages) & 1u;
+        stage0 = y % kStages;
       }
-      if (lane == 0 && any && (!ok || *abort_flag)) {
+      if (any && (!ok || *abort_flag)) {
         volatile uint32_t no_abort = 0;
-        mma_commit(drain);
-        mbar_wait(drain, 0u, &no_abort, c.err);
+        if (elect_one()) {
+          mma_commit(drain);
+          mbar_wait(drain, 0u, &no_abort, c.err);
+        }
+        __syncwarp();
       }
-      __syncwarp();
     }
   } else {
     // -------------------------------------------------------------------- softmax and output
