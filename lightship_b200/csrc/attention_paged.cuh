@@ -39,8 +39,14 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
-// mbar_wait by all lanes of a warp with one outcome (false for all when it ran out for one).
+// mbar_wait by all lanes of a warp with one outcome (false for all when it ran out for one).  The
+// barrier is tried a number of times before mbar_wait starts its clock: reading the global timer
+// takes longer than most waits here.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* err) {
+  const uint32_t at = smem_u32(bar);
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (__all_sync(0xffffffffu, mbar_try_wait(at, parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err)) != 0;
 }
 

@@ -12,18 +12,20 @@
 //   warps 0-3, 4-7  softmax of row tile 0 and 1: thread = row.  S (128 keys) comes from TMEM into
 //                   registers, p goes back to TMEM, packed, in place of S;
 //   warp 8          issues the products: S = Q K^T (A and B in shared memory) and O += P V (A in
-//                   TMEM, V MN-major), the two row tiles in turn, so that one tile's softmax runs
-//                   beside the other's products;
+//                   TMEM, V MN-major), P part by part as the softmax writes it; the row tiles take
+//                   turns, so that one's softmax runs beside the other's products;
 //   warp 9          brings Q and the K and V tiles by TMA, page by page (boxes of pages without a
 //                   visible place read out of the tensor's range: zeros, no traffic);
-//   warp 10         zeroes the rows of V that no row of the unit sees (a product with p = 0 would
-//                   keep a NaN), in the few tiles that have such rows, before they are released;
-//   warp 11         finds the units.
+//   warp 11         finds the units, and zeroes the rows of V that no row of the unit sees (a product
+//                   with p = 0 would keep a NaN) in the few tiles that have such rows, before they
+//                   are released to the products.
 // m moves only when a row's maximum passes it by more than 2^8: until then p stays below 2^8,
 // which the 16-bit types and the f32 sums hold as exactly as values below 1, and O needs no
 // rescaling.  When it moves, the softmax thread rescales its row of O in TMEM; the products into O
 // that it follows are complete, because S of this tile was issued behind them.
 // Every wait is bounded (a timeout flags the device error word and ends the CTA's work).
+#include <type_traits>
+
 #include "attention_paged.cuh"
 
 namespace lsc {
@@ -32,7 +34,38 @@ namespace {
 constexpr int kTile = 128;            // rows of a row tile, places of a key tile
 constexpr int kPrefillThreads = 384;
 constexpr int kSchedSlots = 4;
+constexpr int kParts = 2;              // parts of P that are passed on, of 64 keys each
+constexpr int kPolyEvery = 4;          // of the exponentials, one pair in so many on the FMA units
 constexpr float kMoveBy = 8.0f;       // log2 of how far a maximum may pass the reference
+
+// max of three (NaN operands are ignored)
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of two values on the FMA units, beside the special function unit, which gives 16 a clock and
+// bounds the kernel: x = n + f with n the nearest integer (by adding 1.5 * 2^23 + 127, which leaves
+// n + 127 in the low bits) and |f| <= 1/2; 2^f by the polynomial of degree 5 with the smallest
+// relative error there, 7.5e-8 (found by Remez' exchange); 2^n by its exponent field.  x below
+// -126 counts as -126; NaN stays NaN.
+__device__ __forceinline__ uint64_t exp2_fma(uint64_t x2) {
+  constexpr float kMagic = 12582912.0f + 127.0f;
+  float a, b;
+  f2unpack(x2, a, b);
+  const uint64_t x = f2pack(fmax_nan(a, -126.0f), fmax_nan(b, -126.0f));
+  const uint64_t t = f2add(x, f2pack(kMagic, kMagic));
+  const uint64_t f = f2sub(x, f2sub(t, f2pack(kMagic, kMagic)));
+  uint64_t p = f2pack(0.0013276472454890609f, 0.0013276472454890609f);
+  p = f2fma(p, f, f2pack(0.009675540961325169f, 0.009675540961325169f));
+  p = f2fma(p, f, f2pack(0.05550713092088699f, 0.05550713092088699f));
+  p = f2fma(p, f, f2pack(0.24022120237350464f, 0.24022120237350464f));
+  p = f2fma(p, f, f2pack(0.6931469440460205f, 0.6931469440460205f));
+  p = f2fma(p, f, f2pack(1.0000001192092896f, 1.0000001192092896f));
+  f2unpack(t, a, b);
+  return f2mul(p, f2pack(__uint_as_float(__float_as_uint(a) << 23), __uint_as_float(__float_as_uint(b) << 23)));
+}
 
 template <int D>
 struct PrefillShape {
@@ -66,10 +99,6 @@ struct TileRows {
     first = u.pos0 + w * p.tpt;
     last = first + count - 1;
     low = p.a.window > 0 && first >= p.a.window ? first - p.a.window + 1 : 0;
-  }
-  __device__ __forceinline__ bool meets(int32_t tile, int32_t sinks) const {
-    const int32_t j0 = tile * kTile;
-    return count > 0 && j0 <= last && (j0 + kTile > low || j0 < sinks);
   }
 };
 
@@ -171,7 +200,9 @@ struct Scheduler {
         k -= have;
         continue;
       }
-      const int src = __fns(mask, 0, k + 1);
+      uint32_t rest = mask;
+      for (; k > 0; --k) rest &= rest - 1;
+      const int src = __ffs(rest) - 1;
       const int32_t first = (lo - base) * p.unit_tokens;
       r.b = b0 + src;
       r.row0 = __shfl_sync(0xffffffffu, begin + first, src);
@@ -205,8 +236,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   uint64_t* q_full = landed + kStages;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* o_full = p_full + 2;
+  uint64_t* p_full = s_full + 2;  // [row tile][part]
+  uint64_t* o_full = p_full + 2 * kParts;
   uint64_t* drain = o_full + 2;
   uint64_t* sched_full = drain + 1;
   uint64_t* sched_empty = sched_full + kSchedSlots;
@@ -223,16 +254,16 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       mbar_init(landed + s, 1);
     }
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);
     for (int w = 0; w < 2; ++w) {
       mbar_init(s_full + w, 1);
-      mbar_init(p_full + w, 4);
+      for (int x = 0; x < kParts; ++x) mbar_init(p_full + w * kParts + x, 4);
       mbar_init(o_full + w, 1);
     }
     mbar_init(drain, 1);
     for (int s = 0; s < kSchedSlots; ++s) {
       mbar_init(sched_full + s, 1);
-      mbar_init(sched_empty + s, 11);  // eight softmax warps, products, loads, zeroing
+      mbar_init(sched_empty + s, 10);  // eight softmax warps, products, loads
     }
     *abort_flag = 0u;
     fence_barrier_init();
@@ -269,7 +300,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   if (warp >= 8) {
     regs_shrink<88>();
     if (warp == 11) {
-      // ------------------------------------------------------------------ scheduler
+      // ------------------------------------------------------------------ units, zeroing of unseen V rows
       if (blockIdx.x == 0) {
         int32_t begin, end;
         for (int b = lane; b < c.batch; b += 32) {
@@ -278,25 +309,63 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         }
       }
       const Scheduler s(c, p, lane);
-      bool ok = true;
-      for (int64_t k = 0; ok; ++k) {
-        const int64_t i = k * gridDim.x + ((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        Unit u{};
-        u.b = -1;
-        const bool more = k * gridDim.x < s.total;
-        if (more && i >= s.total) continue;  // this round's part is missing; the last round
-        if (more) u = s.find(i);
-        if (!(ok = warp_wait(sched_empty + sched_at, sched_phase ^ 1u, abort_flag, c.err))) break;
-        if (lane == 0) {
-          sched[sched_at] = u;
-          mbar_arrive(sched_full + sched_at);
+      int64_t round = 0;         // of the next unit to find: the grid walks them to and fro
+      int found = 0, zeroed = 0; // units passed on; units whose V rows are done
+      bool more = true, ok = true;
+      uint32_t stage = 0, land_phase = 0;  // land_phase: one parity bit per stage
+      while (ok && (more || zeroed < found)) {
+        // Pass on the next unit as soon as its slot is free, but wait for a slot only when there is
+        // nothing to zero: the others need no more from this warp to free one.
+        // A slot is not used again before this warp has zeroed its unit.
+        if (more && found - zeroed < kSchedSlots &&
+            (zeroed == found ||
+             __all_sync(0xffffffffu, mbar_test_wait(smem_u32(sched_empty + sched_at), sched_phase ^ 1u)))) {
+          const int64_t i = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+          ++round;
+          Unit u{};
+          u.b = -1;
+          if (i < s.total) u = s.find(i);
+          else if ((round - 1) * gridDim.x < s.total) continue;  // the last round has no unit for this CTA
+          more = u.b >= 0;
+          if (!(ok = warp_wait(sched_empty + sched_at, sched_phase ^ 1u, abort_flag, c.err))) break;
+          if (lane == 0) {
+            sched[sched_at] = u;
+            mbar_arrive(sched_full + sched_at);
+          }
+          __syncwarp();
+          if (++sched_at == kSchedSlots) {
+            sched_at = 0;
+            sched_phase ^= 1u;
+          }
+          if (more) ++found;
+          continue;
         }
-        __syncwarp();
-        if (++sched_at == kSchedSlots) {
-          sched_at = 0;
-          sched_phase ^= 1u;
+        const Unit u = sched[zeroed % kSchedSlots];
+        ++zeroed;
+        const TileList<kTile> tiles = tiles_of(u);
+        const int32_t last = u.pos0 + u.count - 1;
+        const int32_t low = a.window > 0 && u.pos0 >= a.window ? u.pos0 - a.window + 1 : 0;
+        for (int32_t i = 0; i < tiles.n; ++i) {
+          const int32_t j0 = tiles.tile(i) * kTile;
+          const bool whole = j0 + kTile <= last + 1 && (j0 >= low || j0 + kTile <= a.sinks);
+          if (++stage >= kStages) stage -= kStages;  // past the K tile
+          if (!whole) {
+            if (!(ok = warp_wait(landed + stage, (land_phase >> stage) & 1u, abort_flag, c.err))) break;
+            land_phase ^= 1u << stage;
+            uint8_t* v = s_kv + stage * Shape::kTileBytes;
+            // lanes 8 x .. 8 x + 7 write the eight 16-byte parts of row x (of four at a time)
+            for (int r = lane >> 3; r < kTile; r += 4) {
+              if (key_visible(j0 + r, last, low, a.sinks)) continue;
+#pragma unroll
+              for (int x = 0; x < kBlocks; ++x)
+                *reinterpret_cast<uint4*>(v + x * kBlockBytes + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(kv_full + stage);
+          }
+          if (++stage >= kStages) stage -= kStages;
         }
-        if (!more) break;
       }
     } else if (warp == 9) {
       // ------------------------------------------------------------------ loads (whole warp)
@@ -376,134 +445,122 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           else mbar_wait(kv_full + s, (uses - 1) & 1u, &no_abort, c.err);
         }
       }
-    } else if (warp == 10) {
-      // ------------------------------------------------------------------ zeroing of unseen V rows
-      uint32_t stage = 0, land_phase = 0;  // one parity bit per stage
-      bool ok = true;
-      Unit u;
-      while (ok && next_unit(u)) {
-        const TileList<kTile> tiles = tiles_of(u);
-        const int32_t last = u.pos0 + u.count - 1;
-        const int32_t low = a.window > 0 && u.pos0 >= a.window ? u.pos0 - a.window + 1 : 0;
-        for (int32_t i = 0; i < tiles.n; ++i) {
-          const int32_t j0 = tiles.tile(i) * kTile;
-          const bool whole = j0 + kTile <= last + 1 && (j0 >= low || j0 + kTile <= a.sinks);
-          if (++stage >= kStages) stage -= kStages;  // past the K tile
-          if (!whole) {
-            if (!(ok = warp_wait(landed + stage, (land_phase >> stage) & 1u, abort_flag, c.err))) break;
-            land_phase ^= 1u << stage;
-            uint8_t* v = s_kv + stage * Shape::kTileBytes;
-            // lanes 8 x .. 8 x + 7 write the eight 16-byte parts of row x (of four at a time)
-            for (int r = lane >> 3; r < kTile; r += 4) {
-              const int32_t j = j0 + r;
-              if (j <= last && (j >= low || j < a.sinks)) continue;
-#pragma unroll
-              for (int x = 0; x < kBlocks; ++x)
-                *reinterpret_cast<uint4*>(v + x * kBlockBytes + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(kv_full + stage);
-          }
-          if (++stage >= kStages) stage -= kStages;
-        }
-      }
-    } else {
+    } else if (warp == 8) {
       // ------------------------------------------------------------------ products
       // The whole warp walks the tiles and one elected lane issues: a lane that has left its warp
-      // issues at half the rate.  Descriptors are a 64-bit base plus constants.
+      // issues at half the rate.  The warp shares its scheduler with two softmax warps, so what it
+      // computes between a wait and the products behind it counts: addresses are made before the
+      // waits, and what describes the unit is made uniform (the descriptors then stay in uniform
+      // registers).
       constexpr uint32_t idesc_s = BF16 ? idesc_bf16(128, kTile) : idesc_f16(128, kTile);
       constexpr uint32_t idesc_o = (BF16 ? idesc_bf16(128, D) : idesc_f16(128, D)) | (1u << 16);  // V MN-major
+      constexpr uint32_t kDescTile = Shape::kTileBytes >> 4;
       const uint64_t dq = smem_desc_sw128_kmajor(smem_u32(s_q));
       const uint64_t dk = smem_desc_sw128_kmajor(smem_u32(s_kv));
       const uint64_t dv = smem_desc_sw128_mnmajor(smem_u32(s_kv), kBlockBytes);
       uint32_t q_phase = 0, p_phase[2] = {0, 0};
-      uint32_t stage0 = 0, phase0 = 0;  // of the unit's first K tile
+      uint32_t stage = 0, phase = 0;  // of the next K tile that has not been used
       bool ok = true, any = false;
+      auto uniform = [](int32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+      auto step = [](uint32_t& s, uint32_t& ph, uint32_t by) {
+        s += by;
+        if (s >= kStages) {
+          s -= kStages;
+          ph ^= 1u;
+        }
+      };
+      // A commit holds up the issuing lane for about as long as three products, so there is one per
+      // row tile and key tile, behind its scores.  The softmax warps, which wait for it, give back the
+      // stages that it shows to be free.
+      auto issue_scores = [&](int w, uint64_t dka) {  // by the elected lane
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          constexpr int kStep = 32 >> 4, kBlock = kBlockBytes >> 4;
+          mma_f16(tmem + Shape::kColS + w * kTile, dq + w * kDescTile + (k >> 2) * kBlock + (k & 3) * kStep,
+                  dka + (k >> 2) * kBlock + (k & 3) * kStep, idesc_s, k != 0 ? 1u : 0u);
+        }
+        mma_commit(s_full + w);
+      };
       Unit u;
       while (ok && next_unit(u)) {
         const TileList<kTile> tiles = tiles_of(u);
-        if (tiles.n == 0) continue;
-        const TileSpan span[2] = {TileSpan(TileRows(p, u, 0), tiles, a.sinks), TileSpan(TileRows(p, u, 1), tiles, a.sinks)};
-        // stage and phase of tile `x` (K tiles even, V tiles odd) of the unit
-        auto at = [&](int32_t x, uint32_t& stage, uint32_t& phase) {
-          const uint32_t y = stage0 + static_cast<uint32_t>(x);
-          stage = y % kStages;
-          phase = phase0 ^ ((y / kStages) & 1u);
-        };
-        // S of row tile w and tile i; `last`: Q is not needed after it
-        auto scores = [&](int w, int32_t i, bool last) -> bool {
-          uint32_t stage, phase;
-          at(2 * i, stage, phase);
-          if (!warp_wait(kv_full + stage, phase, abort_flag, c.err)) return false;
-          tc_fence_after();
-          const uint64_t dka = dk + stage * (Shape::kTileBytes >> 4);
-          const uint64_t dqa = dq + w * (Shape::kTileBytes >> 4);
-          if (elect_one()) {
+        const int32_t n = uniform(tiles.n);
+        if (n == 0) continue;
+        TileSpan span[2] = {TileSpan(TileRows(p, u, 0), tiles, a.sinks), TileSpan(TileRows(p, u, 1), tiles, a.sinks)};
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              constexpr int kStep = 32 >> 4, kBlock = kBlockBytes >> 4;
-              mma_f16(tmem + Shape::kColS + w * kTile, dqa + (k >> 2) * kBlock + (k & 3) * kStep,
-                      dka + (k >> 2) * kBlock + (k & 3) * kStep, idesc_s, k != 0 ? 1u : 0u);
-            }
-            mma_commit(s_full + w);
-            mma_commit(kv_empty + stage);
-            if (last) mma_commit(q_empty);
-          }
-          __syncwarp();
-          any = true;
-          return true;
-        };
+        for (int w = 0; w < 2; ++w) {
+          span[w].kept = uniform(span[w].kept);
+          span[w].from = uniform(span[w].from);
+          span[w].to = uniform(span[w].to);
+          span[w].n = n;
+        }
         if (!(ok = warp_wait(q_full, q_phase, abort_flag, c.err))) break;
         q_phase ^= 1u;
-        int open = 0;  // row tiles that still have scores to come
         uint32_t more[2] = {0, 0};
-        const int32_t first[2] = {span[0].next(-1), span[1].next(-1)};
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
-          if (first[w] < tiles.n && span[w].next(first[w]) < tiles.n) ++open;
-        if (first[0] < tiles.n) ok = scores(0, first[0], open == 0 && first[1] >= tiles.n);
-        if (ok && first[1] < tiles.n) ok = scores(1, first[1], open == 0);
-        for (int32_t i = 0; i < tiles.n && ok; ++i) {
-          uint32_t stage, phase;
-          at(2 * i + 1, stage, phase);
+        for (int w = 0; w < 2; ++w) {
+          const int32_t first = span[w].next(-1);
+          if (!ok) break;
+          if (first >= n) {
+            if (lane == 0) mbar_arrive(q_empty);  // no softmax warp will
+            __syncwarp();
+            continue;
+          }
+          uint32_t s = stage, ph = phase;
+          for (int32_t i = 0; i < first; ++i) step(s, ph, 2);
+          if (!(ok = warp_wait(kv_full + s, ph, abort_flag, c.err))) break;
+          tc_fence_after();
+          if (elect_one()) issue_scores(w, dk + s * kDescTile);
+          __syncwarp();
+          any = true;
+        }
+        for (int32_t i = 0; i < n && ok; ++i) {
+          uint32_t vs = stage, vph = phase, ks = stage, kph = phase;
+          step(vs, vph, 1);
+          step(ks, kph, 2);
+          const uint64_t dva = dv + vs * kDescTile;
+          if (!(ok = warp_wait(kv_full + vs, vph, abort_flag, c.err))) break;
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
             if (!ok) break;
             if (!span[w].has(i)) {
               if (lane == 0) {
-                mbar_arrive(kv_empty + (stage == 0 ? kStages - 1 : stage - 1));
                 mbar_arrive(kv_empty + stage);
+                mbar_arrive(kv_empty + vs);
               }
               __syncwarp();
               continue;
             }
-            if (!(ok = warp_wait(p_full + w, p_phase[w], abort_flag, c.err))) break;
-            p_phase[w] ^= 1u;
-            if (!(ok = warp_wait(kv_full + stage, phase, abort_flag, c.err))) break;
-            tc_fence_after();
-            const uint64_t dva = dv + stage * (Shape::kTileBytes >> 4);
             const int32_t j = span[w].next(i);
-            if (elect_one()) {
+            uint32_t s = ks, ph = kph;
+            for (int32_t x = i + 1; x < j; ++x) step(s, ph, 2);
+            const uint64_t dka = dk + s * kDescTile;
+            auto products = [&](auto part) {  // by the elected lane
+              constexpr int kSteps = kTile / 16 / kParts, x = decltype(part)::value;
 #pragma unroll
-              for (int k = 0; k < kTile / 16; ++k)
+              for (int k = x * kSteps; k < (x + 1) * kSteps; ++k)
                 mma_f16_ts(tmem + Shape::kColO + w * D, tmem + Shape::kColS + w * kTile + k * 8, dva + k * (2048 >> 4),
                            idesc_o, k != 0 ? 1u : more[w]);
-              mma_commit(kv_empty + stage);
-              if (j >= tiles.n) mma_commit(o_full + w);
+            };
+            if (!(ok = warp_wait(p_full + w * kParts, p_phase[w], abort_flag, c.err))) break;
+            tc_fence_after();
+            if (elect_one()) products(std::integral_constant<int, 0>{});
+            __syncwarp();
+            if (j < n && !(ok = warp_wait(kv_full + s, ph, abort_flag, c.err))) break;
+            if (!(ok = warp_wait(p_full + w * kParts + 1, p_phase[w], abort_flag, c.err))) break;
+            tc_fence_after();
+            if (elect_one()) {
+              products(std::integral_constant<int, 1>{});
+              // S of the row tile's next tile follows its products into O, which read P in S's place
+              if (j < n) issue_scores(w, dka);
+              else mma_commit(o_full + w);
             }
             __syncwarp();
+            p_phase[w] ^= 1u;
             more[w] = 1;
-            if (j < tiles.n) {
-              const bool end = span[w].next(j) >= tiles.n;
-              if (end) --open;
-              ok = scores(w, j, end && open == 0);
-            }
           }
+          step(stage, phase, 2);
         }
-        const uint32_t y = stage0 + 2u * static_cast<uint32_t>(tiles.n);
-        phase0 ^= (y / kStages) & 1u;
-        stage0 = y % kStages;
       }
       if (any && (!ok || *abort_flag)) {
         volatile uint32_t no_abort = 0;
@@ -525,12 +582,20 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     const int token = row / p.hp, head = row - token * p.hp;
     const float scale = a.scale_log2;
     uint32_t s_phase = 0, o_phase = 0;
+    uint32_t stage0 = 0;  // of the unit's first K tile
     Unit u;
     bool ok = true;
     while (ok && next_unit(u)) {
       const TileList<kTile> tiles = tiles_of(u);
       const TileRows rows(p, u, w);
+      const uint32_t unit_stage = stage0;
+      stage0 = (stage0 + 2u * static_cast<uint32_t>(tiles.n)) % kStages;
       if (rows.count == 0) continue;
+      // gives K tile i (v = 0) or V tile i (v = 1) of the unit back to the loads
+      auto release = [&](int32_t i, uint32_t v) {
+        mbar_arrive(kv_empty + (unit_stage + 2u * static_cast<uint32_t>(i) + v) % kStages);
+      };
+      const TileSpan span(rows, tiles, a.sinks);
       const bool mine = token < rows.count;
       // positions of this row and of the warp's first and last one
       const int32_t pos = rows.first + (mine ? token : rows.count - 1);
@@ -539,33 +604,48 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       float ref = -INFINITY;  // the reference m, in units of the raw scores
       float l = 0.0f;
       int done = 0;
-      for (int32_t i = 0; i < tiles.n; ++i) {
+      int32_t before = -1;  // the tile before i
+      for (int32_t i = span.next(-1); i < tiles.n; i = span.next(i)) {
         const int32_t j0 = tiles.tile(i) * kTile;
-        if (!rows.meets(tiles.tile(i), a.sinks)) continue;
         if (!(ok = warp_wait(s_full + w, s_phase, abort_flag, c.err))) break;
         s_phase ^= 1u;
         tc_fence_after();
-        uint32_t s[4][32];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_ld_32x32b_x32(t_s + 32 * x, s[x]);
-        tmem_ld_wait();
-        if (j0 + kTile - 1 > pos_min || (j0 < low_max && j0 + kTile > a.sinks)) {
-          // some row of the warp does not see the whole tile
-#pragma unroll
+        if (quarter == 0 && lane == 0) {
+          // with these scores all products issued before them are complete
+          release(i, 0);
+          if (before >= 0) release(before, 1);
+          if (span.next(i) >= tiles.n) mbar_arrive(q_empty);
+        }
+        before = i;
+        const bool edge = j0 + kTile - 1 > pos_min || (j0 < low_max && j0 + kTile > a.sinks);
+        if (edge) {
+          // some row of the warp does not see the whole tile: -inf in the places it does not see
+#pragma unroll 1
           for (int x = 0; x < 4; ++x) {
             const uint32_t see = visible_mask(j0 + 32 * x, pos, low, a.sinks);
+            uint32_t s[32];
+            tmem_ld_32x32b_x32(t_s + 32 * x, s);
+            tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) s[x][e] = (see >> e) & 1u ? s[x][e] : 0xFF800000u;
+            for (int e = 0; e < 32; ++e) s[e] = (see >> e) & 1u ? s[e] : 0xFF800000u;
+            tmem_st_32x32b_x32(t_s + 32 * x, s);
           }
+          tmem_st_wait();
         }
-        float top[4];
+        float m = -INFINITY;
+#pragma unroll 1
+        for (int h = 0; h < kParts; ++h) {
+          uint32_t s[2][32];
+          tmem_ld_32x32b_x32(t_s + 64 * h, s[0]);
+          tmem_ld_32x32b_x32(t_s + 64 * h + 32, s[1]);
+          tmem_ld_wait();
+          float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          top[x] = __uint_as_float(s[x][0]);
-#pragma unroll
-          for (int e = 1; e < 32; ++e) top[x] = fmaxf(top[x], __uint_as_float(s[x][e]));
+          for (int e = 0; e < 64; e += 2)
+            top[(e >> 1) & 3] =
+                fmax3(top[(e >> 1) & 3], __uint_as_float(s[e >> 5][e & 31]), __uint_as_float(s[e >> 5][(e & 31) + 1]));
+          m = fmax3(fmaxf(top[0], top[1]), top[2], top[3]);
         }
-        const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         if (done == 0) {
           ref = m;
         } else {
@@ -575,7 +655,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             const float f = move ? ex2_approx((ref - m) * scale) : 1.0f;
             if (move) ref = m;
             l *= f;
-#pragma unroll
+#pragma unroll 1
             for (int x = 0; x < D / 32; ++x) {
               uint32_t o[32];
               tmem_ld_32x32b_x32(t_o + 32 * x, o);
@@ -590,24 +670,41 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         const float shift = ref == -INFINITY ? 0.0f : -ref * scale;
         const uint64_t scale2 = f2pack(scale, scale), shift2 = f2pack(shift, shift);
         uint64_t sum2[2] = {0ull, 0ull};
+        // p of the tile, part by part (rolled: the loops of the softmax and of the products together
+        // have to stay in the instruction cache next to the scheduler).  MIXED: every fourth pair on the
+        // FMA units; a tile with masked places keeps to the special function unit, whose 2^-inf is 0.
+        auto exps = [&](auto mixed) {
+#pragma unroll 1
+          for (int h = 0; h < kParts; ++h) {
+            uint32_t s[2][32];
+            tmem_ld_32x32b_x32(t_s + 64 * h, s[0]);
+            tmem_ld_32x32b_x32(t_s + 64 * h + 32, s[1]);
+            tmem_ld_wait();
+            uint32_t packed[32];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t packed[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            float y0, y1;
-            f2unpack(f2fma(f2pack(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), scale2, shift2), y0, y1);
-            y0 = ex2_approx(y0);
-            y1 = ex2_approx(y1);
-            sum2[e & 1] = f2add(sum2[e & 1], f2pack(y0, y1));
-            packed[e] = pack16<BF16>(y0, y1);
+            for (int e = 0; e < 32; ++e) {
+              const int x = e >> 4, y = 2 * (e & 15);
+              const uint64_t y2 = f2fma(f2pack(__uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1])), scale2, shift2);
+              float y0, y1;
+              if (decltype(mixed)::value && e % kPolyEvery == kPolyEvery - 1) {
+                f2unpack(exp2_fma(y2), y0, y1);
+              } else {
+                f2unpack(y2, y0, y1);
+                y0 = ex2_approx(y0);
+                y1 = ex2_approx(y1);
+              }
+              sum2[e & 1] = f2add(sum2[e & 1], f2pack(y0, y1));
+              packed[e] = pack16<BF16>(y0, y1);
+            }
+            tmem_st_32x32b_x32(t_s + 32 * h, packed);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + w * kParts + h);
           }
-          tmem_st_32x32b_x16(t_s + 16 * x, packed);
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + w);
+        };
+        if (edge) exps(std::false_type{});
+        else exps(std::true_type{});
         float s0, s1;
         f2unpack(f2add(sum2[0], sum2[1]), s0, s1);
         l += s0 + s1;
@@ -617,10 +714,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         if (!(ok = warp_wait(o_full + w, o_phase, abort_flag, c.err))) break;
         o_phase ^= 1u;
         tc_fence_after();
+        if (quarter == 0 && lane == 0) release(before, 1);
       }
       const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
       const int64_t at = (static_cast<int64_t>(u.row0 + w * p.tpt + token) * a.q_heads + u.head0 + head) * D;
-#pragma unroll
+#pragma unroll 1
       for (int x = 0; x < D / 32; ++x) {
         uint32_t o[32];
         if (done) {
