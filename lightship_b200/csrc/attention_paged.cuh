@@ -39,15 +39,37 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
-// mbar_wait by all lanes of a warp with one outcome (false for all when it ran out for one).  The
-// barrier is tried a number of times before mbar_wait starts its clock: reading the global timer
-// takes longer than most waits here.
+// mbarrier.try_wait that may suspend the thread for up to a millisecond: a waiting warp that comes
+// back sooner spends issue slots that the softmax needs.
+__device__ __forceinline__ bool mbar_try_wait_long(uint32_t bar_addr, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred P;\n mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n"
+      " selp.u32 %0, 1, 0, P;\n}\n"
+      : "=r"(ok)
+      : "r"(bar_addr), "r"(parity), "r"(1000000u)
+      : "memory");
+  return ok != 0;
+}
+
+// mbar_wait by all lanes of a warp with one outcome (false for all when it ran out).  The global
+// timer takes longer to read than most waits here last, so it is read at every 64th try only; the
+// loop is kept small because it stands in many places.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t* err) {
   const uint32_t at = smem_u32(bar);
+  unsigned long long until = 0;
 #pragma unroll 1
-  for (int i = 0; i < 64; ++i)
-    if (__all_sync(0xffffffffu, mbar_try_wait(at, parity))) return true;
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err)) != 0;
+  for (uint32_t n = 1; !__all_sync(0xffffffffu, mbar_try_wait_long(at, parity)); ++n) {
+    if ((n & 63u) != 0) continue;
+    const unsigned long long now = globaltimer_ns();
+    if (until == 0) until = now + kWaitLimitNs;
+    if (__any_sync(0xffffffffu, *abort_flag != 0 || now > until)) {
+      *abort_flag = 1u;
+      if (now > until) atomicOr(err, LSC_DEVERR_TIMEOUT);
+      return false;
+    }
+  }
+  return true;
 }
 
 // {lo, hi} rounded to the cache's type and packed

@@ -11,12 +11,12 @@
 // grid, which spreads the causal triangle evenly:
 //   warps 0-3, 4-7  softmax of row tile 0 and 1: thread = row.  S (128 keys) comes from TMEM into
 //                   registers, p goes back to TMEM, packed, in place of S;
-//   warp 8          issues the products: S = Q K^T (A and B in shared memory) and O += P V (A in
-//                   TMEM, V MN-major), P part by part as the softmax writes it; the row tiles take
-//                   turns, so that one's softmax runs beside the other's products;
-//   warp 9          brings Q and the K and V tiles by TMA, page by page (boxes of pages without a
-//                   visible place read out of the tensor's range: zeros, no traffic);
-//   warp 11         finds the units, and zeroes the rows of V that no row of the unit sees (a product
+//   warps 8, 9      issue the products of row tile 0 and 1: S = Q K^T (A and B in shared memory) and
+//                   O += P V (A in TMEM, V MN-major), P part by part as the softmax writes it, so
+//                   that one tile's softmax runs beside the other's products;
+//   warp 11         brings the K and V tiles by TMA, page by page; boxes of pages without a visible
+//                   place read out of the tensor's range: zeros, no traffic;
+//   warp 10         finds the units, brings their Q, and zeroes the rows of V that no row of the unit sees (a product
 //                   with p = 0 would keep a NaN) in the few tiles that have such rows, before they
 //                   are released to the products.
 // m moves only when a row's maximum passes it by more than 2^8: until then p stays below 2^8,
@@ -35,7 +35,7 @@ constexpr int kTile = 128;            // rows of a row tile, places of a key til
 constexpr int kPrefillThreads = 384;
 constexpr int kSchedSlots = 4;
 constexpr int kParts = 2;              // parts of P that are passed on, of 64 keys each
-constexpr int kPolyEvery = 4;          // of the exponentials, one pair in so many on the FMA units
+constexpr int kTurnAt = 3;             // the quarter of the exponentials after which the other row tile may begin
 constexpr float kMoveBy = 8.0f;       // log2 of how far a maximum may pass the reference
 
 // max of three (NaN operands are ignored)
@@ -45,33 +45,11 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
-// 2^x of two values on the FMA units, beside the special function unit, which gives 16 a clock and
-// bounds the kernel: x = n + f with n the nearest integer (by adding 1.5 * 2^23 + 127, which leaves
-// n + 127 in the low bits) and |f| <= 1/2; 2^f by the polynomial of degree 5 with the smallest
-// relative error there, 7.5e-8 (found by Remez' exchange); 2^n by its exponent field.  x below
-// -126 counts as -126; NaN stays NaN.
-__device__ __forceinline__ uint64_t exp2_fma(uint64_t x2) {
-  constexpr float kMagic = 12582912.0f + 127.0f;
-  float a, b;
-  f2unpack(x2, a, b);
-  const uint64_t x = f2pack(fmax_nan(a, -126.0f), fmax_nan(b, -126.0f));
-  const uint64_t t = f2add(x, f2pack(kMagic, kMagic));
-  const uint64_t f = f2sub(x, f2sub(t, f2pack(kMagic, kMagic)));
-  uint64_t p = f2pack(0.0013276472454890609f, 0.0013276472454890609f);
-  p = f2fma(p, f, f2pack(0.009675540961325169f, 0.009675540961325169f));
-  p = f2fma(p, f, f2pack(0.05550713092088699f, 0.05550713092088699f));
-  p = f2fma(p, f, f2pack(0.24022120237350464f, 0.24022120237350464f));
-  p = f2fma(p, f, f2pack(0.6931469440460205f, 0.6931469440460205f));
-  p = f2fma(p, f, f2pack(1.0000001192092896f, 1.0000001192092896f));
-  f2unpack(t, a, b);
-  return f2mul(p, f2pack(__uint_as_float(__float_as_uint(a) << 23), __uint_as_float(__float_as_uint(b) << 23)));
-}
-
 template <int D>
 struct PrefillShape {
   static constexpr int kTileBytes = kTile * D * 2;    // Q, K or V of one tile
-  static constexpr int kStages = D == 128 ? 5 : 8;    // K and V tiles in turn
-  static constexpr int kBarBytes = 512;
+  static constexpr int kStages = D == 128 ? 5 : 10;   // K and V tiles in turn
+  static constexpr int kBarBytes = 768;
   static constexpr int kSmem = (2 + kStages) * kTileBytes + kBarBytes + 1024;
   static constexpr uint32_t kColS = 0, kColO = 256;   // TMEM columns: S of both tiles, then O of both
 };
@@ -147,6 +125,7 @@ struct Scheduler {
   }
   __device__ __forceinline__ int64_t at_or_above(int32_t t) const {
     int64_t f = 0;
+#pragma unroll 1
     for (int b = lane; b < c.batch; b += 32) {
       int32_t begin, n, base, count, len;
       of(b, begin, n, base, count, len);
@@ -159,6 +138,7 @@ struct Scheduler {
   }
   __device__ __forceinline__ Scheduler(const PagedView& c_, const PrefillArgs& p_, int lane_)
       : c(c_), p(p_), lane(lane_), top(0) {
+#pragma unroll 1
     for (int b = lane; b < c.batch; b += 32) {
       int32_t begin, n, base, count, len;
       of(b, begin, n, base, count, len);
@@ -190,6 +170,7 @@ struct Scheduler {
     // the (u - F(lo + 1))-th sequence with a unit at level lo
     int32_t k = static_cast<int32_t>(u - above);
     Unit r{};
+#pragma unroll 1
     for (int b0 = 0; b0 < c.batch; b0 += 32) {
       int32_t begin = 0, n = 0, base = 0, count = 0, len = 0;
       if (b0 + lane < c.batch) of(b0 + lane, begin, n, base, count, len);
@@ -239,7 +220,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   uint64_t* p_full = s_full + 2;  // [row tile][part]
   uint64_t* o_full = p_full + 2 * kParts;
   uint64_t* drain = o_full + 2;
-  uint64_t* sched_full = drain + 1;
+  uint64_t* turn = drain + 2;  // [row tile]: the other one has done its exponentials
+  uint64_t* sched_full = turn + 2;
   uint64_t* sched_empty = sched_full + kSchedSlots;
   Unit* sched = reinterpret_cast<Unit*>(sched_empty + kSchedSlots);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sched + kSchedSlots);
@@ -260,10 +242,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       for (int x = 0; x < kParts; ++x) mbar_init(p_full + w * kParts + x, 4);
       mbar_init(o_full + w, 1);
     }
-    mbar_init(drain, 1);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(drain + w, 1);
+      mbar_init(turn + w, 4);
+    }
     for (int s = 0; s < kSchedSlots; ++s) {
       mbar_init(sched_full + s, 1);
-      mbar_init(sched_empty + s, 10);  // eight softmax warps, products, loads
+      mbar_init(sched_empty + s, 8 + 2 + 1);  // softmax, products, loads of K and V
     }
     *abort_flag = 0u;
     fence_barrier_init();
@@ -299,7 +284,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
 
   if (warp >= 8) {
     regs_shrink<88>();
-    if (warp == 11) {
+    if (warp == 10) {
       // ------------------------------------------------------------------ units, zeroing of unseen V rows
       if (blockIdx.x == 0) {
         int32_t begin, end;
@@ -313,6 +298,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       int found = 0, zeroed = 0; // units passed on; units whose V rows are done
       bool more = true, ok = true;
       uint32_t stage = 0, land_phase = 0;  // land_phase: one parity bit per stage
+      uint32_t q_phase = 0;
+      int q_loads = 0;
       while (ok && (more || zeroed < found)) {
         // Pass on the next unit as soon as its slot is free, but wait for a slot only when there is
         // nothing to zero: the others need no more from this warp to free one.
@@ -343,6 +330,20 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         const Unit u = sched[zeroed % kSchedSlots];
         ++zeroed;
         const TileList<kTile> tiles = tiles_of(u);
+        if (tiles.n == 0) continue;
+        // Q, once the scores of the unit before are done (they need no more from this warp)
+        if (!(ok = warp_wait(q_empty, q_phase ^ 1u, abort_flag, c.err))) break;
+        q_phase ^= 1u;
+        if (lane == 0) {
+          const int q_tiles = u.count > p.tpt ? 2 : 1;
+          mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(q_tiles * kBlocks * p.hp * p.tpt * 128));
+          for (int w = 0; w < q_tiles; ++w)
+            for (int x = 0; x < kBlocks; ++x)
+              tma_load_3d(&tm_q, q_full, s_q + w * Shape::kTileBytes + x * kBlockBytes, x * 64, u.head0,
+                          u.row0 + w * p.tpt);
+        }
+        __syncwarp();
+        ++q_loads;
         const int32_t last = u.pos0 + u.count - 1;
         const int32_t low = a.window > 0 && u.pos0 >= a.window ? u.pos0 - a.window + 1 : 0;
         for (int32_t i = 0; i < tiles.n; ++i) {
@@ -367,16 +368,22 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           if (++stage >= kStages) stage -= kStages;
         }
       }
-    } else if (warp == 9) {
-      // ------------------------------------------------------------------ loads (whole warp)
+      if ((!ok || *abort_flag) && q_loads > 0) {
+        // let the copies in flight land before the CTA exits
+        volatile uint32_t no_abort = 0;
+        mbar_wait(q_full, static_cast<uint32_t>((q_loads - 1) & 1), &no_abort, c.err);
+      }
+    } else if (warp == 11) {
+      // ------------------------------------------------------------------ loads of K and V
+      constexpr int32_t kUnseen = INT32_MIN;  // the page of a box without a visible place
       const int page_size = 1 << c.page_shift;
       const int box_rows = page_size < kTile ? page_size : kTile;
       const int per_tile = kTile / box_rows;
       const int boxes = per_tile * kBlocks;  // at most 32
       const int sub = lane % per_tile, block = lane / per_tile;
-      uint32_t stage = 0, phase = 0, q_phase = 0;
-      uint32_t by_landed = 0, land_parity = 0;  // per stage: how its last tile came, uses of `landed` mod 2
-      int issued = 0, q_loads = 0;
+      uint32_t stage0 = 0, phase0 = 0;  // of the unit's first K tile
+      uint32_t land_parity = 0;         // per stage: uses of `landed` mod 2
+      uint32_t used = 0, by_land = 0, parity = 0;  // per stage: the last copy and its barrier
       bool ok = true;
       Unit u;
       while (ok && next_unit(u)) {
@@ -384,84 +391,73 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         if (tiles.n == 0) continue;
         const int32_t last = u.pos0 + u.count - 1;
         const int32_t low = a.window > 0 && u.pos0 >= a.window ? u.pos0 - a.window + 1 : 0;
-        if (!(ok = warp_wait(q_empty, q_phase ^ 1u, abort_flag, c.err))) break;
-        q_phase ^= 1u;
-        if (lane == 0) {
-          const int q_tiles = u.count > p.tpt ? 2 : 1;
-          mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(q_tiles * kBlocks * p.hp * p.tpt * 128));
-          for (int w = 0; w < q_tiles; ++w)
-            for (int x = 0; x < kBlocks; ++x)
-              tma_load_3d(&tm_q, q_full, s_q + w * Shape::kTileBytes + x * kBlockBytes, x * 64, u.head0,
-                          u.row0 + w * p.tpt);
-        }
-        ++q_loads;
         auto page_of = [&](int32_t i) -> int32_t {
           const int32_t j0 = tiles.tile(i) * kTile + sub * box_rows;
           const bool seen = j0 <= last && (j0 + box_rows > low || j0 < a.sinks);
-          if (!seen) return static_cast<int32_t>(c.num_pages);
-          const int32_t id = __ldg(c.table + u.b * c.table_stride + (j0 >> c.page_shift));
-          if (id >= 0 && id < c.num_pages) return id;
-          raise_bad_arg(c.err);
-          return static_cast<int32_t>(c.num_pages);
+          return seen ? __ldg(c.table + u.b * c.table_stride + (j0 >> c.page_shift)) : kUnseen;
         };
-        int32_t page = page_of(0);
-        for (int32_t i = 0; i < tiles.n && ok; ++i) {
-          const int32_t next = i + 1 < tiles.n ? page_of(i + 1) : 0;
-          const int32_t j0 = tiles.tile(i) * kTile;
-          const bool whole = j0 + kTile <= last + 1 && (j0 >= low || j0 + kTile <= a.sinks);
-#pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            if (!(ok = warp_wait(kv_empty + stage, phase ^ 1u, abort_flag, c.err))) break;
-            uint64_t* bar = (v == 1 && !whole ? landed : kv_full) + stage;
-            if (lane == 0) mbar_arrive_expect_tx(bar, Shape::kTileBytes);
-            __syncwarp();
-            if (lane < boxes)
-              tma_load_4d(v == 1 ? &tm_v : &tm_k, bar,
-                          s_kv + stage * Shape::kTileBytes + block * kBlockBytes + sub * box_rows * 128, block * 64,
-                          (j0 + sub * box_rows) & (page_size - 1), u.kvh, page);
-            ++issued;
-            if (v == 1 && !whole) {
-              by_landed |= 1u << stage;
-              land_parity ^= 1u << stage;
-            } else {
-              by_landed &= ~(1u << stage);
-            }
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1u;
-            }
+        const int32_t count = 2 * tiles.n;  // K tiles even, V tiles odd
+        int32_t next = page_of(0);
+        for (int32_t x = 0; x < count; ++x) {
+          const uint32_t y = stage0 + static_cast<uint32_t>(x);
+          const uint32_t stage = y % kStages, bit = 1u << stage, phase = phase0 ^ ((y / kStages) & 1u);
+          int32_t page = next;
+          if (x + 1 < count) next = page_of((x + 1) >> 1);
+          if (page < 0 || page >= c.num_pages) {
+            if (page != kUnseen) raise_bad_arg(c.err);
+            page = static_cast<int32_t>(c.num_pages);
           }
-          page = next;
+          const int32_t t0 = tiles.tile(x >> 1) * kTile, j0 = t0 + sub * box_rows;
+          const bool by_landed = (x & 1) != 0 && !(t0 + kTile <= last + 1 && (t0 >= low || t0 + kTile <= a.sinks));
+          if (!(ok = warp_wait(kv_empty + stage, phase ^ 1u, abort_flag, c.err))) break;
+          uint64_t* bar = (by_landed ? landed : kv_full) + stage;
+          if (lane == 0) mbar_arrive_expect_tx(bar, Shape::kTileBytes);
+          __syncwarp();
+          if (lane < boxes)
+            tma_load_4d((x & 1) != 0 ? &tm_v : &tm_k, bar,
+                        s_kv + stage * Shape::kTileBytes + block * kBlockBytes + sub * box_rows * 128, block * 64,
+                        j0 & (page_size - 1), u.kvh, page);
+          __syncwarp();
+          used |= bit;
+          if (by_landed) {
+            by_land |= bit;
+            parity = (parity & ~bit) | (land_parity & bit);
+            land_parity ^= bit;
+          } else {
+            by_land &= ~bit;
+            parity = (parity & ~bit) | (phase ? bit : 0u);
+          }
         }
+        const uint32_t y = stage0 + static_cast<uint32_t>(count);
+        phase0 ^= (y / kStages) & 1u;
+        stage0 = y % kStages;
       }
       if (!ok || *abort_flag) {
         // let the copies in flight land before the CTA exits
         volatile uint32_t no_abort = 0;
-        if (q_loads > 0) mbar_wait(q_full, static_cast<uint32_t>((q_loads - 1) & 1), &no_abort, c.err);
-        // (all but a stage's last tile have been used, so they are complete)
-        for (int s = 0; s < kStages && s < issued; ++s) {
-          const uint32_t uses = (issued - s + kStages - 1) / kStages;
-          if ((by_landed >> s) & 1u) mbar_wait(landed + s, ((land_parity >> s) & 1u) ^ 1u, &no_abort, c.err);
-          else mbar_wait(kv_full + s, (uses - 1) & 1u, &no_abort, c.err);
-        }
+        for (int s = 0; s < kStages; ++s)
+          if ((used >> s) & 1u)
+            mbar_wait(((by_land >> s) & 1u ? landed : kv_full) + s, (parity >> s) & 1u, &no_abort, c.err);
       }
-    } else if (warp == 8) {
-      // ------------------------------------------------------------------ products
+    } else {
+      // ------------------------------------------------------------------ products of one row tile
       // The whole warp walks the tiles and one elected lane issues: a lane that has left its warp
-      // issues at half the rate.  The warp shares its scheduler with two softmax warps, so what it
-      // computes between a wait and the products behind it counts: addresses are made before the
-      // waits, and what describes the unit is made uniform (the descriptors then stay in uniform
-      // registers).
+      // issues at half the rate.  One warp per row tile, because what a warp does between products
+      // (waits, addresses, a commit that takes the time of three products) would leave the tensor
+      // pipe idle; what describes the unit is made uniform, so that descriptors stay in uniform
+      // registers.
       constexpr uint32_t idesc_s = BF16 ? idesc_bf16(128, kTile) : idesc_f16(128, kTile);
       constexpr uint32_t idesc_o = (BF16 ? idesc_bf16(128, D) : idesc_f16(128, D)) | (1u << 16);  // V MN-major
       constexpr uint32_t kDescTile = Shape::kTileBytes >> 4;
-      const uint64_t dq = smem_desc_sw128_kmajor(smem_u32(s_q));
+      auto uniform = [](int32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+      const int w = uniform(warp == 8 ? 0 : 1);
+      const uint64_t dq = smem_desc_sw128_kmajor(smem_u32(s_q + w * Shape::kTileBytes));
       const uint64_t dk = smem_desc_sw128_kmajor(smem_u32(s_kv));
       const uint64_t dv = smem_desc_sw128_mnmajor(smem_u32(s_kv), kBlockBytes);
-      uint32_t q_phase = 0, p_phase[2] = {0, 0};
+      const uint32_t t_s = uniform(tmem) + Shape::kColS + w * kTile, t_o = uniform(tmem) + Shape::kColO + w * D;
+      uint32_t q_phase = 0, p_phase = 0;
       uint32_t stage = 0, phase = 0;  // of the next K tile that has not been used
       bool ok = true, any = false;
-      auto uniform = [](int32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
       auto step = [](uint32_t& s, uint32_t& ph, uint32_t by) {
         s += by;
         if (s >= kStages) {
@@ -469,15 +465,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           ph ^= 1u;
         }
       };
-      // A commit holds up the issuing lane for about as long as three products, so there is one per
-      // row tile and key tile, behind its scores.  The softmax warps, which wait for it, give back the
+      // One commit per key tile, behind its scores.  The softmax warps, which wait for it, give back the
       // stages that it shows to be free.
-      auto issue_scores = [&](int w, uint64_t dka) {  // by the elected lane
+      auto issue_scores = [&](uint64_t dka) {  // by the elected lane
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           constexpr int kStep = 32 >> 4, kBlock = kBlockBytes >> 4;
-          mma_f16(tmem + Shape::kColS + w * kTile, dq + w * kDescTile + (k >> 2) * kBlock + (k & 3) * kStep,
-                  dka + (k >> 2) * kBlock + (k & 3) * kStep, idesc_s, k != 0 ? 1u : 0u);
+          mma_f16(t_s, dq + (k >> 2) * kBlock + (k & 3) * kStep, dka + (k >> 2) * kBlock + (k & 3) * kStep, idesc_s,
+                  k != 0 ? 1u : 0u);
         }
         mma_commit(s_full + w);
       };
@@ -486,87 +481,78 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         const TileList<kTile> tiles = tiles_of(u);
         const int32_t n = uniform(tiles.n);
         if (n == 0) continue;
-        TileSpan span[2] = {TileSpan(TileRows(p, u, 0), tiles, a.sinks), TileSpan(TileRows(p, u, 1), tiles, a.sinks)};
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          span[w].kept = uniform(span[w].kept);
-          span[w].from = uniform(span[w].from);
-          span[w].to = uniform(span[w].to);
-          span[w].n = n;
-        }
+        TileSpan span(TileRows(p, u, w), tiles, a.sinks);
+        span.kept = uniform(span.kept);
+        span.from = uniform(span.from);
+        span.to = uniform(span.to);
+        span.n = n;
         if (!(ok = warp_wait(q_full, q_phase, abort_flag, c.err))) break;
         q_phase ^= 1u;
-        uint32_t more[2] = {0, 0};
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int32_t first = span[w].next(-1);
-          if (!ok) break;
-          if (first >= n) {
-            if (lane == 0) mbar_arrive(q_empty);  // no softmax warp will
-            __syncwarp();
-            continue;
-          }
+        uint32_t more = 0;
+        const int32_t first = span.next(-1);
+        if (first < n) {
           uint32_t s = stage, ph = phase;
           for (int32_t i = 0; i < first; ++i) step(s, ph, 2);
           if (!(ok = warp_wait(kv_full + s, ph, abort_flag, c.err))) break;
           tc_fence_after();
-          if (elect_one()) issue_scores(w, dk + s * kDescTile);
+          if (elect_one()) issue_scores(dk + s * kDescTile);
           __syncwarp();
           any = true;
+        } else {
+          if (lane == 0) mbar_arrive(q_empty);  // no softmax warp will
+          __syncwarp();
         }
-        for (int32_t i = 0; i < n && ok; ++i) {
+        for (int32_t i = 0; i < n; ++i) {
           uint32_t vs = stage, vph = phase, ks = stage, kph = phase;
           step(vs, vph, 1);
           step(ks, kph, 2);
-          const uint64_t dva = dv + vs * kDescTile;
           if (!(ok = warp_wait(kv_full + vs, vph, abort_flag, c.err))) break;
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            if (!ok) break;
-            if (!span[w].has(i)) {
-              if (lane == 0) {
-                mbar_arrive(kv_empty + stage);
-                mbar_arrive(kv_empty + vs);
-              }
-              __syncwarp();
-              continue;
-            }
-            const int32_t j = span[w].next(i);
-            uint32_t s = ks, ph = kph;
-            for (int32_t x = i + 1; x < j; ++x) step(s, ph, 2);
-            const uint64_t dka = dk + s * kDescTile;
-            auto products = [&](auto part) {  // by the elected lane
-              constexpr int kSteps = kTile / 16 / kParts, x = decltype(part)::value;
-#pragma unroll
-              for (int k = x * kSteps; k < (x + 1) * kSteps; ++k)
-                mma_f16_ts(tmem + Shape::kColO + w * D, tmem + Shape::kColS + w * kTile + k * 8, dva + k * (2048 >> 4),
-                           idesc_o, k != 0 ? 1u : more[w]);
-            };
-            if (!(ok = warp_wait(p_full + w * kParts, p_phase[w], abort_flag, c.err))) break;
-            tc_fence_after();
-            if (elect_one()) products(std::integral_constant<int, 0>{});
-            __syncwarp();
-            if (j < n && !(ok = warp_wait(kv_full + s, ph, abort_flag, c.err))) break;
-            if (!(ok = warp_wait(p_full + w * kParts + 1, p_phase[w], abort_flag, c.err))) break;
-            tc_fence_after();
-            if (elect_one()) {
-              products(std::integral_constant<int, 1>{});
-              // S of the row tile's next tile follows its products into O, which read P in S's place
-              if (j < n) issue_scores(w, dka);
-              else mma_commit(o_full + w);
+          if (!span.has(i)) {
+            // Not this row tile's: give the stages back once they hold the tile (before, the arrival
+            // would count for the tile that they held last).
+            if (!(ok = warp_wait(kv_full + stage, phase, abort_flag, c.err))) break;
+            if (lane == 0) {
+              mbar_arrive(kv_empty + stage);
+              mbar_arrive(kv_empty + vs);
             }
             __syncwarp();
-            p_phase[w] ^= 1u;
-            more[w] = 1;
+            step(stage, phase, 2);
+            continue;
           }
+          const uint64_t dva = dv + vs * kDescTile;
+          const int32_t j = span.next(i);
+          for (int32_t x = i + 1; x < j; ++x) step(ks, kph, 2);
+          const uint64_t dka = dk + ks * kDescTile;
+          auto products = [&](auto part) {  // by the elected lane
+            constexpr int kSteps = kTile / 16 / kParts, x = decltype(part)::value;
+#pragma unroll
+            for (int k = x * kSteps; k < (x + 1) * kSteps; ++k)
+              mma_f16_ts(t_o, t_s + k * 8, dva + k * (2048 >> 4), idesc_o, k != 0 ? 1u : more);
+          };
+          if (!(ok = warp_wait(p_full + w * kParts, p_phase, abort_flag, c.err))) break;
+          tc_fence_after();
+          if (elect_one()) products(std::integral_constant<int, 0>{});
+          __syncwarp();
+          if (j < n && !(ok = warp_wait(kv_full + ks, kph, abort_flag, c.err))) break;
+          if (!(ok = warp_wait(p_full + w * kParts + 1, p_phase, abort_flag, c.err))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            products(std::integral_constant<int, 1>{});
+            // S of the row tile's next tile follows its products into O, which read P in S's place
+            if (j < n) issue_scores(dka);
+            else mma_commit(o_full + w);
+          }
+          __syncwarp();
+          p_phase ^= 1u;
+          more = 1;
           step(stage, phase, 2);
         }
       }
       if (any && (!ok || *abort_flag)) {
         volatile uint32_t no_abort = 0;
         if (elect_one()) {
-          mma_commit(drain);
-          mbar_wait(drain, 0u, &no_abort, c.err);
+          mma_commit(drain + w);
+          mbar_wait(drain + w, 0u, &no_abort, c.err);
         }
         __syncwarp();
       }
@@ -583,6 +569,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     const float scale = a.scale_log2;
     uint32_t s_phase = 0, o_phase = 0;
     uint32_t stage0 = 0;  // of the unit's first K tile
+    uint32_t turn_phase = w == 0 ? 1u : 0u;  // row tile 0 begins
     Unit u;
     bool ok = true;
     while (ok && next_unit(u)) {
@@ -595,7 +582,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       auto release = [&](int32_t i, uint32_t v) {
         mbar_arrive(kv_empty + (unit_stage + 2u * static_cast<uint32_t>(i) + v) % kStages);
       };
-      const TileSpan span(rows, tiles, a.sinks);
+      const TileSpan span(rows, tiles, a.sinks), other_span(TileRows(p, u, w ^ 1), tiles, a.sinks);
       const bool mine = token < rows.count;
       // positions of this row and of the warp's first and last one
       const int32_t pos = rows.first + (mine ? token : rows.count - 1);
@@ -610,42 +597,28 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         if (!(ok = warp_wait(s_full + w, s_phase, abort_flag, c.err))) break;
         s_phase ^= 1u;
         tc_fence_after();
-        if (quarter == 0 && lane == 0) {
-          // with these scores all products issued before them are complete
-          release(i, 0);
-          if (before >= 0) release(before, 1);
-          if (span.next(i) >= tiles.n) mbar_arrive(q_empty);
-        }
-        before = i;
-        const bool edge = j0 + kTile - 1 > pos_min || (j0 < low_max && j0 + kTile > a.sinks);
-        if (edge) {
+        uint32_t s[4][32];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmem_ld_32x32b_x32(t_s + 32 * x, s[x]);
+        tmem_ld_wait();
+        if (j0 + kTile - 1 > pos_min || (j0 < low_max && j0 + kTile > a.sinks)) {
           // some row of the warp does not see the whole tile: -inf in the places it does not see
-#pragma unroll 1
+#pragma unroll
           for (int x = 0; x < 4; ++x) {
             const uint32_t see = visible_mask(j0 + 32 * x, pos, low, a.sinks);
-            uint32_t s[32];
-            tmem_ld_32x32b_x32(t_s + 32 * x, s);
-            tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) s[e] = (see >> e) & 1u ? s[e] : 0xFF800000u;
-            tmem_st_32x32b_x32(t_s + 32 * x, s);
+            for (int e = 0; e < 32; ++e) s[x][e] = (see >> e) & 1u ? s[x][e] : 0xFF800000u;
           }
-          tmem_st_wait();
         }
-        float m = -INFINITY;
-#pragma unroll 1
-        for (int h = 0; h < kParts; ++h) {
-          uint32_t s[2][32];
-          tmem_ld_32x32b_x32(t_s + 64 * h, s[0]);
-          tmem_ld_32x32b_x32(t_s + 64 * h + 32, s[1]);
-          tmem_ld_wait();
-          float top[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+        float top[4];
 #pragma unroll
-          for (int e = 0; e < 64; e += 2)
-            top[(e >> 1) & 3] =
-                fmax3(top[(e >> 1) & 3], __uint_as_float(s[e >> 5][e & 31]), __uint_as_float(s[e >> 5][(e & 31) + 1]));
-          m = fmax3(fmaxf(top[0], top[1]), top[2], top[3]);
+        for (int x = 0; x < 4; ++x) {
+          top[x] = __uint_as_float(s[x][0]);
+#pragma unroll
+          for (int e = 1; e < 31; e += 2) top[x] = fmax3(top[x], __uint_as_float(s[x][e]), __uint_as_float(s[x][e + 1]));
+          top[x] = fmaxf(top[x], __uint_as_float(s[x][31]));
         }
+        const float m = fmax3(fmaxf(top[0], top[1]), top[2], top[3]);
         if (done == 0) {
           ref = m;
         } else {
@@ -670,41 +643,43 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         const float shift = ref == -INFINITY ? 0.0f : -ref * scale;
         const uint64_t scale2 = f2pack(scale, scale), shift2 = f2pack(shift, shift);
         uint64_t sum2[2] = {0ull, 0ull};
-        // p of the tile, part by part (rolled: the loops of the softmax and of the products together
-        // have to stay in the instruction cache next to the scheduler).  MIXED: every fourth pair on the
-        // FMA units; a tile with masked places keeps to the special function unit, whose 2^-inf is 0.
-        auto exps = [&](auto mixed) {
-#pragma unroll 1
-          for (int h = 0; h < kParts; ++h) {
-            uint32_t s[2][32];
-            tmem_ld_32x32b_x32(t_s + 64 * h, s[0]);
-            tmem_ld_32x32b_x32(t_s + 64 * h + 32, s[1]);
-            tmem_ld_wait();
-            uint32_t packed[32];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int x = e >> 4, y = 2 * (e & 15);
-              const uint64_t y2 = f2fma(f2pack(__uint_as_float(s[x][y]), __uint_as_float(s[x][y + 1])), scale2, shift2);
-              float y0, y1;
-              if (decltype(mixed)::value && e % kPolyEvery == kPolyEvery - 1) {
-                f2unpack(exp2_fma(y2), y0, y1);
-              } else {
-                f2unpack(y2, y0, y1);
-                y0 = ex2_approx(y0);
-                y1 = ex2_approx(y1);
-              }
-              sum2[e & 1] = f2add(sum2[e & 1], f2pack(y0, y1));
-              packed[e] = pack16<BF16>(y0, y1);
-            }
-            tmem_st_32x32b_x32(t_s + 32 * h, packed);
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full + w * kParts + h);
-          }
+        // The two row tiles take turns at the special function units: in step with each other they would
+        // wait for them together and for the products together.
+        const bool shared = other_span.has(i);
+        if (shared) {
+          if (!(ok = warp_wait(turn + w, turn_phase, abort_flag, c.err))) break;
+          turn_phase ^= 1u;
+        }
+        auto arrive = [&](int part) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full + w * kParts + part);
         };
-        if (edge) exps(std::false_type{});
-        else exps(std::true_type{});
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float y0, y1;
+            f2unpack(f2fma(f2pack(__uint_as_float(s[x][2 * e]), __uint_as_float(s[x][2 * e + 1])), scale2, shift2), y0, y1);
+            y0 = ex2_approx(y0);
+            y1 = ex2_approx(y1);
+            sum2[e & 1] = f2add(sum2[e & 1], f2pack(y0, y1));
+            packed[e] = pack16<BF16>(y0, y1);
+          }
+          if (shared && x == kTurnAt && lane == 0) mbar_arrive(turn + (w ^ 1));
+          if (x == 2) arrive(0);  // its stores have had the time of 32 keys to complete
+          tmem_st_32x32b_x16(t_s + 16 * x, packed);
+        }
+        arrive(1);
+        if (quarter == 0 && lane == 0) {
+          // with the scores all products issued before them were complete
+          release(i, 0);
+          if (before >= 0) release(before, 1);
+          if (span.next(i) >= tiles.n) mbar_arrive(q_empty);
+        }
+        before = i;
         float s0, s1;
         f2unpack(f2add(sum2[0], sum2[1]), s0, s1);
         l += s0 + s1;
@@ -719,35 +694,32 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
       const int64_t at = (static_cast<int64_t>(u.row0 + w * p.tpt + token) * a.q_heads + u.head0 + head) * D;
 #pragma unroll 1
-      for (int x = 0; x < D / 32; ++x) {
-        uint32_t o[32];
+      for (int x = 0; x < D / 16; ++x) {
+        uint32_t o[16];
         if (done) {
-          tmem_ld_32x32b_x32(t_o + 32 * x, o);
+          tmem_ld_32x32b_x16(t_o + 16 * x, o);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
+          for (int e = 0; e < 16; ++e) o[e] = 0u;
         }
         __syncwarp();
         if (mine) {
-        float y[32];
+          float y[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * inv;
-        if (a.out) {
+          for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(o[e]) * inv;
+          if (a.out) {
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
-            *reinterpret_cast<uint4*>(a.out + at + 32 * x + 8 * v) =
-                make_uint4(pack16<BF16>(y[8 * v], y[8 * v + 1]), pack16<BF16>(y[8 * v + 2], y[8 * v + 3]),
-                           pack16<BF16>(y[8 * v + 4], y[8 * v + 5]), pack16<BF16>(y[8 * v + 6], y[8 * v + 7]));
-        }
-        if (a.out_i8) {
-          uint32_t pk[8];
-          requant_pack<32>(y, a.s_out, a.inv_s_out, false, a.rounding, pk);
-#pragma unroll
-          for (int v = 0; v < 2; ++v)
-            *reinterpret_cast<uint4*>(a.out_i8 + at + 32 * x + 16 * v) =
-                make_uint4(pk[4 * v], pk[4 * v + 1], pk[4 * v + 2], pk[4 * v + 3]);
-        }
+            for (int v = 0; v < 2; ++v)
+              *reinterpret_cast<uint4*>(a.out + at + 16 * x + 8 * v) =
+                  make_uint4(pack16<BF16>(y[8 * v], y[8 * v + 1]), pack16<BF16>(y[8 * v + 2], y[8 * v + 3]),
+                             pack16<BF16>(y[8 * v + 4], y[8 * v + 5]), pack16<BF16>(y[8 * v + 6], y[8 * v + 7]));
+          }
+          if (a.out_i8) {
+            uint32_t pk[4];
+            requant_pack<16>(y, a.s_out, a.inv_s_out, false, a.rounding, pk);
+            *reinterpret_cast<uint4*>(a.out_i8 + at + 16 * x) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          }
         }
         __syncwarp();
       }

@@ -140,6 +140,22 @@ def test_prefill(cuda, index, window, sinks, kind):
     ops.check_device()
 
 
+@pytest.mark.parametrize("seqs,heads,group,d,page,window,sinks,kind", [
+    ([(5000, 5000)], 8, 4, 128, 64, 0, 0, "float16"),
+    ([(5000, 5000), (3000, 100), (1, 1), (2222, 2222)], 8, 2, 128, 16, 700, 9, "bfloat16"),
+    ([(6000, 4000)], 6, 3, 64, 32, 300, 4, "float16"),
+    ([(100 + 13 * i, 100) for i in range(60)], 4, 4, 64, 8, 0, 0, "bfloat16"),
+])
+def test_prefill_more_units_than_sms(cuda, seqs, heads, group, d, page, window, sinks, kind):
+    """Many units of work for each SM, one after another."""
+    from lightship_b200 import ops
+    cache, q, offsets, keys, values = make(seqs, heads, group, d, page, kind, seed=11)
+    for _ in range(3):
+        out = cache.prefill(q, offsets, window=window, sinks=sinks)
+    check(out, q, offsets, keys, values, seqs, kind, window, sinks)
+    ops.check_device()
+
+
 @pytest.mark.parametrize("kind", ["float16", "bfloat16"])
 @pytest.mark.parametrize("window,sinks", MASKS)
 @pytest.mark.parametrize("seqs,heads,group,d,page", [
