@@ -174,6 +174,8 @@ _lock = threading.Lock()
 def lib() -> C.CDLL:
     """Loads the CUDA backend library (raises if it has not been built)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):

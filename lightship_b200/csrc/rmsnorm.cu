@@ -1,9 +1,18 @@
 // rmsnorm.cu -- root-mean-square norm of the rows of [rows, d] with the residual's addition and an
 // int8 output (static scale, or one scale per row):
 //   h = x + r;  y = (h / sqrt(mean(h^2) + eps)) * gamma;  q = clamp(R(y / s), -128, 127)
-// One CTA per row; sums in f32.
+// Each element is read once and written once, with about five flops, so HBM bounds it.
+//
+// Rows whose buffers are all 16-byte aligned and whose length is a multiple of 8, up to 16384: the
+// row stays in registers (h as f32, 8 elements a thread and step), so nothing is read twice; the
+// sum of squares is reduced over the row's threads, and the largest |h gamma| with it when the row
+// finds its own scale.  TPR threads share a row, from a warp for short rows to 512 for the longest,
+// so that a thread holds at most 32 elements; short rows share a CTA.
+// Any other row (odd lengths, odd strides, longer ones) is walked twice by one CTA.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "epilogue.cuh"
 #include "lsc_internal.h"
@@ -11,7 +20,9 @@
 namespace lsc {
 namespace {
 
-constexpr int kRmsThreads = 256;
+constexpr int kWalkThreads = 256;
+constexpr int kVec = 8;            // elements of a vector step
+constexpr int kMaxRow = 16384;     // elements of a row held in registers
 
 struct RmsArgs {
   const void* x;
@@ -23,7 +34,7 @@ struct RmsArgs {
   float* row_scales;
   int64_t x_stride, res_stride, sum_stride, out_stride, q_stride;
   int64_t rows, d;
-  float eps, s_out;
+  float eps, s_out, inv_s_out;
   int32_t rounding;
 };
 
@@ -34,43 +45,211 @@ __device__ __forceinline__ void st1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void st1(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void st1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <typename TX, typename TR>
-__global__ void __launch_bounds__(kRmsThreads) rmsnorm_kernel(const RmsArgs a) {
-  __shared__ float red[2 * kRmsThreads / 32];
+// Eight elements at a 16-byte aligned address, as loaded and as f32
+template <typename T>
+struct Raw {
+  uint4 v[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> load8(const T* p) {
+  Raw<T> r;
+  r.v[0] = *reinterpret_cast<const uint4*>(p);
+  if constexpr (sizeof(T) == 4) r.v[1] = *reinterpret_cast<const uint4*>(p + 4);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void widen(const Raw<T>& r, float (&f)[kVec]) {
+  const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t u[4] = {r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f[e] = __uint_as_float(w[e]);
+      f[4 + e] = __uint_as_float(u[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float2 v;
+      if constexpr (std::is_same<T, __half>::value) v = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+      else v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
+      f[2 * e] = v.x;
+      f[2 * e + 1] = v.y;
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&f)[kVec]) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(f[2 * e], f[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * e], f[2 * e + 1]);
+        w[e] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// The row's scale from its largest |y|: find_scale_zp's symmetric rule.
+__device__ __forceinline__ float row_scale(float top) { return top > 0.0f ? __fdiv_rn(top, 127.0f) : 1.0f; }
+
+// Rows in registers: TPR threads per row, STEPS vectors of 8 elements per thread (element
+// (step * TPR + thread) * 8).
+template <typename TX, typename TR, int TPR, int STEPS>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, STEPS <= 2 ? (TPR < 512 ? 4 : 2) : 1)
+    rmsnorm_rows_kernel(const RmsArgs a) {
+  constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR, kWarps = TPR / 32;
+  __shared__ float red[2][kThreads / 32];
+  griddep_wait();
+  griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int in_row = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const int d = static_cast<int>(a.d);
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kRows; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * kRows) {
+    const int64_t r = r0 + sub;
+    const bool live = r < a.rows;
+    const TX* x = static_cast<const TX*>(a.x) + r * a.x_stride;
+    const TR* res = static_cast<const TR*>(a.res) + r * a.res_stride;
+    Raw<TX> xr[STEPS];
+    Raw<TR> rr[STEPS];
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int i = (s * TPR + in_row) * kVec;
+      if (live && i < d) {
+        xr[s] = load8(x + i);
+        if (a.res) rr[s] = load8(res + i);
+      }
+    }
+    float h[STEPS][kVec];
+    float ss = 0.0f, top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int i = (s * TPR + in_row) * kVec;
+      if (live && i < d) {
+        widen(xr[s], h[s]);
+        if (a.res) {
+          float f[kVec];
+          widen(rr[s], f);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) h[s][e] = __fadd_rn(h[s][e], f[e]);
+          if (a.sum_out) store8(static_cast<TR*>(a.sum_out) + r * a.sum_stride + i, h[s]);
+        }
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) ss = fmaf(h[s][e], h[s][e], ss);
+        if (a.row_scales) {
+          float g[kVec] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
+          if (a.gamma) widen(load8(a.gamma + i), g);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) top = fmaxf(top, fabsf(h[s][e] * g[e]));
+        }
+      }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (a.row_scales) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    if constexpr (kWarps > 1) {
+      __syncthreads();  // the row before has been read
+      if (lane == 0) {
+        red[0][warp] = ss;
+        red[1][warp] = top;
+      }
+      __syncthreads();
+      ss = 0.0f;
+      top = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        ss += red[0][sub * kWarps + w];
+        top = fmaxf(top, red[1][sub * kWarps + w]);
+      }
+    }
+    if (!live) continue;
+    const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(d)), a.eps)));
+    float scale = a.s_out, inv_scale = a.inv_s_out;
+    if (a.row_scales) {
+      scale = row_scale(top * inv);
+      // a reciprocal that is not a normal number sends every value to the division
+      inv_scale = scale >= 1.2e-38f && scale <= 8.0e37f ? __frcp_rn(scale) : 0.0f;
+      if (in_row == 0) a.row_scales[r] = scale;
+    }
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int i = (s * TPR + in_row) * kVec;
+      if (i < d) {
+        float y[kVec];
+        if (a.gamma) {
+          float g[kVec];
+          widen(load8(a.gamma + i), g);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) y[e] = h[s][e] * inv * g[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) y[e] = h[s][e] * inv;
+        }
+        if (a.out) store8(static_cast<TX*>(a.out) + r * a.out_stride + i, y);
+        if (a.q) {
+          uint32_t pk[2];
+          requant_pack<kVec>(y, scale, inv_scale, false, a.rounding, pk);
+          *reinterpret_cast<uint2*>(a.q + r * a.q_stride + i) = make_uint2(pk[0], pk[1]);
+        }
+      }
+    }
+  }
+}
+
+// Any row: one CTA walks it twice.
+template <typename TX, typename TR>
+__global__ void __launch_bounds__(kWalkThreads) rmsnorm_walk_kernel(const RmsArgs a) {
+  __shared__ float red[2][kWalkThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  griddep_wait();
+  griddep_launch_dependents();
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const TX* x = static_cast<const TX*>(a.x) + r * a.x_stride;
     const TR* res = a.res ? static_cast<const TR*>(a.res) + r * a.res_stride : nullptr;
     float ss = 0.0f, top = 0.0f;
-    for (int64_t i = threadIdx.x; i < a.d; i += kRmsThreads) {
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < a.d; i += kWalkThreads) {
       const float h = res ? __fadd_rn(ld1(x + i), ld1(res + i)) : ld1(x + i);
       ss = fmaf(h, h, ss);
       top = fmaxf(top, fabsf(a.gamma ? h * __ldg(a.gamma + i) : h));
     }
+#pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       ss += __shfl_xor_sync(0xffffffffu, ss, o);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
     __syncthreads();
     if (lane == 0) {
-      red[warp] = ss;
-      red[kRmsThreads / 32 + warp] = top;
+      red[0][warp] = ss;
+      red[1][warp] = top;
     }
     __syncthreads();
     ss = 0.0f;
     top = 0.0f;
-    for (int w = 0; w < kRmsThreads / 32; ++w) {
-      ss += red[w];
-      top = fmaxf(top, red[kRmsThreads / 32 + w]);
+#pragma unroll
+    for (int w = 0; w < kWalkThreads / 32; ++w) {
+      ss += red[0][w];
+      top = fmaxf(top, red[1][w]);
     }
     const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(a.d)), a.eps)));
     float s = a.s_out;
     if (a.row_scales) {
-      const float am = top * inv;
-      s = am > 0.0f ? __fdiv_rn(am, 127.0f) : 1.0f;
+      s = row_scale(top * inv);
       if (threadIdx.x == 0) a.row_scales[r] = s;
     }
-    for (int64_t i = threadIdx.x; i < a.d; i += kRmsThreads) {
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < a.d; i += kWalkThreads) {
       const float h = res ? __fadd_rn(ld1(x + i), ld1(res + i)) : ld1(x + i);
       const float y = a.gamma ? h * inv * __ldg(a.gamma + i) : h * inv;
       if (a.sum_out) st1(static_cast<TR*>(a.sum_out) + r * a.sum_stride + i, h);
@@ -83,11 +262,31 @@ __global__ void __launch_bounds__(kRmsThreads) rmsnorm_kernel(const RmsArgs a) {
   }
 }
 
+template <typename TX, typename TR, int TPR, int STEPS>
+lsc_status launch_rows(const RmsArgs& a, const DeviceState* ds, cudaStream_t st) {
+  constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
+  const int64_t ctas = (a.rows + kRows - 1) / kRows;
+  const int64_t cap = static_cast<int64_t>(ds->sm_count) * 32;
+  LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, rmsnorm_rows_kernel<TX, TR, TPR, STEPS>,
+                                dim3(static_cast<unsigned>(ctas < cap ? ctas : cap)), dim3(kThreads), 0, st, a));
+  return LSC_SUCCESS;
+}
+
 template <typename TX, typename TR>
-lsc_status launch(const RmsArgs& a, int sm_count, cudaStream_t st) {
-  const int64_t cap = static_cast<int64_t>(sm_count) * 8;
-  rmsnorm_kernel<TX, TR><<<static_cast<int>(a.rows < cap ? a.rows : cap), kRmsThreads, 0, st>>>(a);
-  LSC_CUDA_TRY(cudaGetLastError());
+lsc_status launch(const RmsArgs& a, const DeviceState* ds, bool vectors, cudaStream_t st) {
+  if (vectors) {
+    const int64_t v = a.d / kVec;  // vectors of a row
+    if (v <= 32) return launch_rows<TX, TR, 32, 1>(a, ds, st);
+    if (v <= 64) return launch_rows<TX, TR, 64, 1>(a, ds, st);
+    if (v <= 128) return launch_rows<TX, TR, 64, 2>(a, ds, st);
+    if (v <= 256) return launch_rows<TX, TR, 128, 2>(a, ds, st);
+    if (v <= 512) return launch_rows<TX, TR, 256, 2>(a, ds, st);
+    if (v <= 1024) return launch_rows<TX, TR, 512, 2>(a, ds, st);
+    return launch_rows<TX, TR, 512, 4>(a, ds, st);
+  }
+  const int64_t cap = static_cast<int64_t>(ds->sm_count) * 8;
+  LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, rmsnorm_walk_kernel<TX, TR>,
+                                dim3(static_cast<unsigned>(a.rows < cap ? a.rows : cap)), dim3(kWalkThreads), 0, st, a));
   return LSC_SUCCESS;
 }
 
@@ -148,14 +347,24 @@ extern "C" lsc_status lsc_rmsnorm(const void* x, int32_t x_dtype, int64_t x_stri
   a.eps = eps;
   a.s_out = s_out;
   a.rounding = rounding;
+  a.inv_s_out = out_i8 && !row_scales ? reciprocal_or_zero(s_out) : 0.0f;
+  // every vector of 8 elements aligned: bases on 16 bytes, strides multiples of 8 elements (an int8
+  // row's vectors are 8 bytes)
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) |
+                          reinterpret_cast<uintptr_t>(sum_out) | reinterpret_cast<uintptr_t>(out) |
+                          reinterpret_cast<uintptr_t>(gamma) | (reinterpret_cast<uintptr_t>(out_i8) << 1);
+  const int64_t strides = rows > 1 ? x_stride | (residual ? residual_stride : 0) | (sum_out ? sum_stride : 0) |
+                                         (out ? out_stride : 0) | (out_i8 ? i8_stride : 0)
+                                   : 0;
+  const bool vectors = d <= kMaxRow && d % kVec == 0 && bases % 16 == 0 && strides % kVec == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool wide = residual && residual_dtype == LSC_DTYPE_F32;
   switch (x_dtype) {
-    case LSC_DTYPE_F32: return launch<float, float>(a, ds->sm_count, st);
+    case LSC_DTYPE_F32: return launch<float, float>(a, ds, vectors, st);
     case LSC_DTYPE_F16:
-      return wide ? launch<__half, float>(a, ds->sm_count, st) : launch<__half, __half>(a, ds->sm_count, st);
+      return wide ? launch<__half, float>(a, ds, vectors, st) : launch<__half, __half>(a, ds, vectors, st);
     default:
-      return wide ? launch<__nv_bfloat16, float>(a, ds->sm_count, st)
-                  : launch<__nv_bfloat16, __nv_bfloat16>(a, ds->sm_count, st);
+      return wide ? launch<__nv_bfloat16, float>(a, ds, vectors, st)
+                  : launch<__nv_bfloat16, __nv_bfloat16>(a, ds, vectors, st);
   }
 }

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .ops import _DTYPES, _on, _stream
+from .ops import _DTYPES, _on, _raw_stream
 
 
 class PagedKVCache:
@@ -54,6 +54,8 @@ class PagedKVCache:
             *k.stride()[:3], page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(), page_table.shape[1],
             self.batch)
         self._ref = C.byref(self._desc)
+        self._scale = self.head_dim ** -0.5
+        self._workspace_bytes = {}  # by query heads
 
     def _heads(self, t, name):
         """A [tokens, heads, head_dim] tensor of the cache's type with contiguous heads."""
@@ -81,7 +83,7 @@ class PagedKVCache:
         with _on(self.device):
             check(lib().lsc_kv_cache_append(self._ref, k_new.data_ptr(), v_new.data_ptr(), k_new.shape[0],
                                             k_new.stride(0), k_new.stride(1), q_offsets.data_ptr(),
-                                            _stream(self.device)))
+                                            _raw_stream(self.device)))
 
     def _outputs(self, q, out, out_i8):
         if out is None and out_i8 is None:
@@ -105,15 +107,17 @@ class PagedKVCache:
         with _on(self.device):
             check(lib().lsc_paged_attention_prefill(
                 self._ref, q.data_ptr(), q.shape[0], q.shape[1], q.stride(0), q.stride(1), q_offsets.data_ptr(),
-                self.head_dim ** -0.5 if alpha is None else alpha, window, sinks,
+                self._scale if alpha is None else alpha, window, sinks,
                 None if out is None else out.data_ptr(), None if out_i8 is None else out_i8.data_ptr(), s_out,
-                rounding, _stream(self.device)))
+                rounding, _raw_stream(self.device)))
         return out if out is not None else out_i8
 
     def decode_workspace(self, q_heads):
         """A workspace for ``decode`` with that many query heads."""
-        with _on(self.device):
+        n = self._workspace_bytes.get(q_heads)
+        if n is None:
             n = lib().lsc_paged_attention_decode_workspace_size(self._ref, q_heads)
+            self._workspace_bytes[q_heads] = n
         return torch.empty(n, dtype=torch.uint8, device=self.device)
 
     def decode(self, q, alpha=None, window=0, sinks=0, out=None, out_i8=None, s_out=1.0,
@@ -133,8 +137,8 @@ class PagedKVCache:
         with _on(self.device):
             check(lib().lsc_paged_attention_decode(
                 self._ref, q.data_ptr(), q.shape[1], q.stride(0), q.stride(1),
-                self.head_dim ** -0.5 if alpha is None else alpha, window, sinks,
+                self._scale if alpha is None else alpha, window, sinks,
                 None if out is None else out.data_ptr(), None if out_i8 is None else out_i8.data_ptr(), s_out,
                 rounding, workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-                _stream(self.device)))
+                _raw_stream(self.device)))
         return out if out is not None else out_i8

@@ -141,17 +141,15 @@ def attention_f16(qkv, batch, seq, heads, alpha=0.125, out_f32=None, out_i8=None
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 
 
-def _rows(t, dtype, name, like=None):
-    """A CUDA tensor of rows whose elements are contiguous: (pointer, row stride)."""
-    if t is None:
-        return None, 0
-    if t.dim() != 2 or not t.is_cuda or t.dtype != dtype or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name}: expected a 2-D CUDA {dtype} tensor with contiguous rows, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}, strides {t.stride()}")
-    if like is not None and (t.shape != like.shape or t.device != like.device):
-        raise ValueError(f"{name}: shape {tuple(t.shape)} on {t.device} does not match {tuple(like.shape)} on "
-                         f"{like.device}")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _rows(t, dtype, name, shape, device):
+    """Checks a 2-D CUDA tensor of rows whose elements are contiguous: (pointer, row stride)."""
+    if t.dtype != dtype or t.shape != shape or t.device != device:
+        raise ValueError(f"{name}: expected a {dtype} tensor of {tuple(shape)} on {device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    row, element = t.stride()
+    if element != 1 and shape[1] > 1:
+        raise ValueError(f"{name}: the elements of a row must be contiguous, strides {t.stride()}")
+    return t.data_ptr(), row if shape[0] > 1 else shape[1]
 
 
 def rmsnorm(x, gamma=None, eps=1e-5, residual=None, sum_out=None, out=None, out_i8=None, s_out=0.0,
@@ -165,31 +163,41 @@ def rmsnorm(x, gamma=None, eps=1e-5, residual=None, sum_out=None, out=None, out_
     ([rows] f32) is given to receive them.  With neither ``out`` nor ``out_i8``, ``out`` is
     allocated.  Returns ``out`` if there is one, else ``out_i8``.
     """
-    code = _DTYPES.get(x.dtype)
-    if code is None:
-        raise ValueError(f"x: expected f32, f16 or bf16, got {x.dtype}")
-    px, sx = _rows(x, x.dtype, "x")
+    dtype, shape, device = x.dtype, x.shape, x.device
+    code = _DTYPES.get(dtype)
+    if code is None or not x.is_cuda or len(shape) != 2:
+        raise ValueError(f"x: expected a 2-D CUDA f32, f16 or bf16 tensor, got {dtype} {tuple(shape)} on {device}")
+    px, sx = _rows(x, dtype, "x", shape, device)
     if out is None and out_i8 is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    rcode = code
+        out = torch.empty(shape, dtype=dtype, device=device)
+    rtype, rcode, pr, sr, ps, ss, po, so, pq, sq = dtype, code, None, 0, None, 0, None, 0, None, 0
     if residual is not None:
-        if residual.dtype != x.dtype and residual.dtype != torch.float32:
-            raise ValueError(f"residual: expected {x.dtype} or f32, got {residual.dtype}")
-        rcode = _DTYPES[residual.dtype]
-    pr, sr = _rows(residual, None if residual is None else residual.dtype, "residual", x)
-    ps, ss = _rows(sum_out, x.dtype if residual is None else residual.dtype, "sum_out", x)
-    po, so = _rows(out, x.dtype, "out", x)
-    pq, sq = _rows(out_i8, torch.int8, "out_i8", x)
-    rows, d = x.shape
-    for name, t, n in (("gamma", gamma, d), ("row_scales", row_scales, rows)):
-        if t is not None:
-            _need(t, torch.float32, name)
-            if t.numel() != n or t.device != x.device:
-                raise ValueError(f"{name}: expected {n} values on {x.device}")
-    with _on(x.device):
-        check(lib().lsc_rmsnorm(px, code, sx, pr, rcode, sr, rows, d, _ptr(gamma), float(eps), ps, ss, po, so, pq, sq,
-                                float(s_out), _ptr(row_scales), int(rounding), _stream(x.device)))
+        rtype = residual.dtype
+        if rtype != dtype and rtype != torch.float32:
+            raise ValueError(f"residual: expected {dtype} or f32, got {rtype}")
+        rcode = _DTYPES[rtype]
+        pr, sr = _rows(residual, rtype, "residual", shape, device)
+    if sum_out is not None:
+        ps, ss = _rows(sum_out, rtype, "sum_out", shape, device)
+    if out is not None:
+        po, so = _rows(out, dtype, "out", shape, device)
+    if out_i8 is not None:
+        pq, sq = _rows(out_i8, torch.int8, "out_i8", shape, device)
+    for name, t, n in (("gamma", gamma, shape[1]), ("row_scales", row_scales, shape[0])):
+        if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.device != device or
+                              not t.is_contiguous()):
+            raise ValueError(f"{name}: expected {n} contiguous f32 values on {device}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+    with _on(device):
+        check(lib().lsc_rmsnorm(px, code, sx, pr, rcode, sr, shape[0], shape[1],
+                                None if gamma is None else gamma.data_ptr(), eps, ps, ss, po, so, pq, sq, s_out,
+                                None if row_scales is None else row_scales.data_ptr(), rounding, _raw_stream(device)))
     return out if out is not None else out_i8
+
+
+def _raw_stream(device):
+    """The current stream's handle as an int (torch's accessor without the Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 class _Here:
