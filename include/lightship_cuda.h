@@ -510,8 +510,8 @@ lsc_status lsc_paged_attention_prefill(const lsc_paged_kv* cache, const void* q,
  * kv_lens[b] - 1; an empty sequence gives zeros): the cache's length is split over the GPU and
  * the parts are joined in a fixed order, so results do not change from run to run.  Places that
  * the row does not see have no effect, whatever they hold.  `workspace`: device scratch of
- * lsc_paged_attention_decode_workspace_size(cache, q_heads) bytes, 16-byte aligned, with any
- * content; calls that share one must be ordered on one stream (two captured graphs that share
+ * lsc_paged_attention_decode_workspace_size(cache, q_heads) bytes (0 where no sequence can hold
+ * more than 512 tokens: then it may be NULL), 16-byte aligned, with any content; calls that share one must be ordered on one stream (two captured graphs that share
  * one must not run at the same time). */
 uint64_t lsc_paged_attention_decode_workspace_size(const lsc_paged_kv* cache, int32_t q_heads);
 lsc_status lsc_paged_attention_decode(const lsc_paged_kv* cache, const void* q, int32_t q_heads,

@@ -3,12 +3,12 @@
 //   h = x + r;  y = (h / sqrt(mean(h^2) + eps)) * gamma;  q = clamp(R(y / s), -128, 127)
 // Each element is read once and written once, with about five flops, so HBM bounds it.
 //
-// Rows whose buffers are all 16-byte aligned and whose length is a multiple of 8, up to 16384: the
-// row stays in registers (h as f32, 8 elements a thread and step), so nothing is read twice; the
-// sum of squares is reduced over the row's threads, and the largest |h gamma| with it when the row
-// finds its own scale.  TPR threads share a row, from a warp for short rows to 512 for the longest,
-// so that a thread holds at most 32 elements; short rows share a CTA.
-// Any other row (odd lengths, odd strides, longer ones) is walked twice by one CTA.
+// Rows of up to 16384 elements stay in registers (h as f32), so nothing is read twice; the sum of
+// squares is reduced over the row's threads, and the largest |h gamma| with it when the row finds
+// its own scale.  TPR threads share a row, from 8 for short rows to 512 for the longest, so that a
+// thread holds at most 32 elements; short rows share a CTA.  A thread takes 8 neighbours at a time
+// where every buffer is 16-byte aligned and the length a multiple of 8, single elements elsewhere.
+// Longer rows are walked twice by one CTA.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -21,7 +21,6 @@ namespace lsc {
 namespace {
 
 constexpr int kWalkThreads = 256;
-constexpr int kVec = 8;            // elements of a vector step
 constexpr int kMaxRow = 16384;     // elements of a row held in registers
 
 struct RmsArgs {
@@ -45,42 +44,56 @@ __device__ __forceinline__ void st1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void st1(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void st1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// Eight elements at a 16-byte aligned address, as loaded and as f32
-template <typename T>
+// V (8 or 1) elements as loaded and as f32; 8 at a 16-byte aligned address
+template <typename T, int V>
 struct Raw {
   uint4 v[sizeof(T) / 2];
 };
 template <typename T>
-__device__ __forceinline__ Raw<T> load8(const T* p) {
-  Raw<T> r;
-  r.v[0] = *reinterpret_cast<const uint4*>(p);
-  if constexpr (sizeof(T) == 4) r.v[1] = *reinterpret_cast<const uint4*>(p + 4);
+struct Raw<T, 1> {
+  T v;
+};
+template <int V, typename T>
+__device__ __forceinline__ Raw<T, V> load(const T* p) {
+  Raw<T, V> r;
+  if constexpr (V == 1) {
+    r.v = *p;
+  } else {
+    r.v[0] = *reinterpret_cast<const uint4*>(p);
+    if constexpr (sizeof(T) == 4) r.v[1] = *reinterpret_cast<const uint4*>(p + 4);
+  }
   return r;
 }
-template <typename T>
-__device__ __forceinline__ void widen(const Raw<T>& r, float (&f)[kVec]) {
-  const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
-  if constexpr (sizeof(T) == 4) {
-    const uint32_t u[4] = {r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      f[e] = __uint_as_float(w[e]);
-      f[4 + e] = __uint_as_float(u[e]);
-    }
+template <int V, typename T>
+__device__ __forceinline__ void widen(const Raw<T, V>& r, float (&f)[V]) {
+  if constexpr (V == 1) {
+    f[0] = ld1(&r.v);
   } else {
+    const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+    if constexpr (sizeof(T) == 4) {
+      const uint32_t u[4] = {r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float2 v;
-      if constexpr (std::is_same<T, __half>::value) v = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-      else v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
-      f[2 * e] = v.x;
-      f[2 * e + 1] = v.y;
+      for (int e = 0; e < 4; ++e) {
+        f[e] = __uint_as_float(w[e]);
+        f[4 + e] = __uint_as_float(u[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float2 v;
+        if constexpr (std::is_same<T, __half>::value) v = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+        else v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[e]));
+        f[2 * e] = v.x;
+        f[2 * e + 1] = v.y;
+      }
     }
   }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[kVec]) {
-  if constexpr (sizeof(T) == 4) {
+template <int V, typename T>
+__device__ __forceinline__ void store(T* p, const float (&f)[V]) {
+  if constexpr (V == 1) {
+    st1(p, f[0]);
+  } else if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
     *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
   } else {
@@ -102,10 +115,10 @@ __device__ __forceinline__ void store8(T* p, const float (&f)[kVec]) {
 // The row's scale from its largest |y|: find_scale_zp's symmetric rule.
 __device__ __forceinline__ float row_scale(float top) { return top > 0.0f ? __fdiv_rn(top, 127.0f) : 1.0f; }
 
-// Rows in registers: TPR threads per row, STEPS vectors of 8 elements per thread (element
-// (step * TPR + thread) * 8).
-template <typename TX, typename TR, int TPR, int STEPS>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, STEPS <= 2 ? (TPR < 512 ? 4 : 2) : 1)
+// Rows in registers: TPR threads per row, STEPS steps of V elements per thread (element
+// (step * TPR + thread) * V).
+template <typename TX, typename TR, int V, int TPR, int STEPS>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, V * STEPS <= 16 ? (TPR < 512 ? 4 : 2) : (TPR < 512 ? 2 : 1))
     rmsnorm_rows_kernel(const RmsArgs a) {
   constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR, kWarps = TPR / 32;
   __shared__ float red[2][kThreads / 32];
@@ -119,42 +132,42 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, STEPS <= 2 ? (TPR < 512
     const bool live = r < a.rows;
     const TX* x = static_cast<const TX*>(a.x) + r * a.x_stride;
     const TR* res = static_cast<const TR*>(a.res) + r * a.res_stride;
-    Raw<TX> xr[STEPS];
-    Raw<TR> rr[STEPS];
+    Raw<TX, V> xr[STEPS];
+    Raw<TR, V> rr[STEPS];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      const int i = (s * TPR + in_row) * kVec;
+      const int i = (s * TPR + in_row) * V;
       if (live && i < d) {
-        xr[s] = load8(x + i);
-        if (a.res) rr[s] = load8(res + i);
+        xr[s] = load<V>(x + i);
+        if (a.res) rr[s] = load<V>(res + i);
       }
     }
-    float h[STEPS][kVec];
+    float h[STEPS][V];
     float ss = 0.0f, top = 0.0f;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
-      const int i = (s * TPR + in_row) * kVec;
+      const int i = (s * TPR + in_row) * V;
       if (live && i < d) {
-        widen(xr[s], h[s]);
+        widen<V>(xr[s], h[s]);
         if (a.res) {
-          float f[kVec];
-          widen(rr[s], f);
+          float f[V];
+          widen<V>(rr[s], f);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) h[s][e] = __fadd_rn(h[s][e], f[e]);
-          if (a.sum_out) store8(static_cast<TR*>(a.sum_out) + r * a.sum_stride + i, h[s]);
+          for (int e = 0; e < V; ++e) h[s][e] = __fadd_rn(h[s][e], f[e]);
+          if (a.sum_out) store<V>(static_cast<TR*>(a.sum_out) + r * a.sum_stride + i, h[s]);
         }
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) ss = fmaf(h[s][e], h[s][e], ss);
+        for (int e = 0; e < V; ++e) ss = fmaf(h[s][e], h[s][e], ss);
         if (a.row_scales) {
-          float g[kVec] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
-          if (a.gamma) widen(load8(a.gamma + i), g);
+          float g[V];
+          if (a.gamma) widen<V>(load<V>(a.gamma + i), g);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) top = fmaxf(top, fabsf(h[s][e] * g[e]));
+          for (int e = 0; e < V; ++e) top = fmaxf(top, fabsf(a.gamma ? h[s][e] * g[e] : h[s][e]));
         }
       }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
       ss += __shfl_xor_sync(0xffffffffu, ss, o);
       if (a.row_scales) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     }
@@ -173,37 +186,46 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, STEPS <= 2 ? (TPR < 512
         top = fmaxf(top, red[1][sub * kWarps + w]);
       }
     }
-    if (!live) continue;
-    const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(d)), a.eps)));
-    float scale = a.s_out, inv_scale = a.inv_s_out;
-    if (a.row_scales) {
-      scale = row_scale(top * inv);
-      // a reciprocal that is not a normal number sends every value to the division
-      inv_scale = scale >= 1.2e-38f && scale <= 8.0e37f ? __frcp_rn(scale) : 0.0f;
-      if (in_row == 0) a.row_scales[r] = scale;
-    }
+    if (live) {
+      const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(d)), a.eps)));
+      float scale = a.s_out, inv_scale = a.inv_s_out;
+      if (a.row_scales) {
+        scale = row_scale(top * inv);
+        // a reciprocal that is not a normal number sends every value to the division
+        inv_scale = scale >= 1.2e-38f && scale <= 8.0e37f ? __frcp_rn(scale) : 0.0f;
+        if (in_row == 0) a.row_scales[r] = scale;
+      }
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const int i = (s * TPR + in_row) * kVec;
-      if (i < d) {
-        float y[kVec];
-        if (a.gamma) {
-          float g[kVec];
-          widen(load8(a.gamma + i), g);
+      for (int s = 0; s < STEPS; ++s) {
+        const int i = (s * TPR + in_row) * V;
+        if (i < d) {
+          float y[V];
+          if (a.gamma) {
+            float g[V];
+            widen<V>(load<V>(a.gamma + i), g);
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) y[e] = h[s][e] * inv * g[e];
-        } else {
+            for (int e = 0; e < V; ++e) y[e] = h[s][e] * inv * g[e];
+          } else {
 #pragma unroll
-          for (int e = 0; e < kVec; ++e) y[e] = h[s][e] * inv;
-        }
-        if (a.out) store8(static_cast<TX*>(a.out) + r * a.out_stride + i, y);
-        if (a.q) {
-          uint32_t pk[2];
-          requant_pack<kVec>(y, scale, inv_scale, false, a.rounding, pk);
-          *reinterpret_cast<uint2*>(a.q + r * a.q_stride + i) = make_uint2(pk[0], pk[1]);
+            for (int e = 0; e < V; ++e) y[e] = h[s][e] * inv;
+          }
+          if (a.out) store<V>(static_cast<TX*>(a.out) + r * a.out_stride + i, y);
+          if (a.q) {
+            int8_t* q = a.q + r * a.q_stride + i;
+            if constexpr (V == 1) {
+              *q = static_cast<int8_t>(a.rounding == LSC_ROUND_HALF_EVEN
+                                           ? requant_one<LSC_ROUND_HALF_EVEN>(y[0], scale, inv_scale)
+                                           : requant_one<LSC_ROUND_HALF_AWAY>(y[0], scale, inv_scale));
+            } else {
+              uint32_t pk[2];
+              requant_pack<8>(y, scale, inv_scale, false, a.rounding, pk);
+              *reinterpret_cast<uint2*>(q) = make_uint2(pk[0], pk[1]);
+            }
+          }
         }
       }
     }
+    __syncwarp();
   }
 }
 
@@ -262,27 +284,37 @@ __global__ void __launch_bounds__(kWalkThreads) rmsnorm_walk_kernel(const RmsArg
   }
 }
 
-template <typename TX, typename TR, int TPR, int STEPS>
+template <typename TX, typename TR, int V, int TPR, int STEPS>
 lsc_status launch_rows(const RmsArgs& a, const DeviceState* ds, cudaStream_t st) {
   constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
   const int64_t ctas = (a.rows + kRows - 1) / kRows;
   const int64_t cap = static_cast<int64_t>(ds->sm_count) * 32;
-  LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, rmsnorm_rows_kernel<TX, TR, TPR, STEPS>,
+  LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, rmsnorm_rows_kernel<TX, TR, V, TPR, STEPS>,
                                 dim3(static_cast<unsigned>(ctas < cap ? ctas : cap)), dim3(kThreads), 0, st, a));
   return LSC_SUCCESS;
 }
 
 template <typename TX, typename TR>
 lsc_status launch(const RmsArgs& a, const DeviceState* ds, bool vectors, cudaStream_t st) {
-  if (vectors) {
-    const int64_t v = a.d / kVec;  // vectors of a row
-    if (v <= 32) return launch_rows<TX, TR, 32, 1>(a, ds, st);
-    if (v <= 64) return launch_rows<TX, TR, 64, 1>(a, ds, st);
-    if (v <= 128) return launch_rows<TX, TR, 64, 2>(a, ds, st);
-    if (v <= 256) return launch_rows<TX, TR, 128, 2>(a, ds, st);
-    if (v <= 512) return launch_rows<TX, TR, 256, 2>(a, ds, st);
-    if (v <= 1024) return launch_rows<TX, TR, 512, 2>(a, ds, st);
-    return launch_rows<TX, TR, 512, 4>(a, ds, st);
+  if (a.d <= kMaxRow && vectors) {
+    const int64_t v = a.d / 8;  // vectors of a row
+    if (v <= 8) return launch_rows<TX, TR, 8, 8, 1>(a, ds, st);
+    if (v <= 16) return launch_rows<TX, TR, 8, 16, 1>(a, ds, st);
+    if (v <= 32) return launch_rows<TX, TR, 8, 32, 1>(a, ds, st);
+    if (v <= 64) return launch_rows<TX, TR, 8, 32, 2>(a, ds, st);
+    if (v <= 96) return launch_rows<TX, TR, 8, 32, 3>(a, ds, st);
+    if (v <= 128) return launch_rows<TX, TR, 8, 64, 2>(a, ds, st);
+    if (v <= 256) return launch_rows<TX, TR, 8, 128, 2>(a, ds, st);
+    if (v <= 512) return launch_rows<TX, TR, 8, 256, 2>(a, ds, st);
+    if (v <= 1024) return launch_rows<TX, TR, 8, 512, 2>(a, ds, st);
+    return launch_rows<TX, TR, 8, 512, 4>(a, ds, st);
+  }
+  if (a.d <= kMaxRow) {
+    if (a.d <= 32) return launch_rows<TX, TR, 1, 8, 4>(a, ds, st);
+    if (a.d <= 256) return launch_rows<TX, TR, 1, 32, 8>(a, ds, st);
+    if (a.d <= 1024) return launch_rows<TX, TR, 1, 128, 8>(a, ds, st);
+    if (a.d <= 4096) return launch_rows<TX, TR, 1, 256, 16>(a, ds, st);
+    return launch_rows<TX, TR, 1, 512, 32>(a, ds, st);
   }
   const int64_t cap = static_cast<int64_t>(ds->sm_count) * 8;
   LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, rmsnorm_walk_kernel<TX, TR>,
@@ -356,7 +388,7 @@ extern "C" lsc_status lsc_rmsnorm(const void* x, int32_t x_dtype, int64_t x_stri
   const int64_t strides = rows > 1 ? x_stride | (residual ? residual_stride : 0) | (sum_out ? sum_stride : 0) |
                                          (out ? out_stride : 0) | (out_i8 ? i8_stride : 0)
                                    : 0;
-  const bool vectors = d <= kMaxRow && d % kVec == 0 && bases % 16 == 0 && strides % kVec == 0;
+  const bool vectors = d % 8 == 0 && bases % 16 == 0 && strides % 8 == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool wide = residual && residual_dtype == LSC_DTYPE_F32;
   switch (x_dtype) {

@@ -141,10 +141,10 @@ def attention_f16(qkv, batch, seq, heads, alpha=0.125, out_f32=None, out_i8=None
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 
 
-def _rows(t, dtype, name, shape, device):
+def _rows(t, dtype, name, shape, index):
     """Checks a 2-D CUDA tensor of rows whose elements are contiguous: (pointer, row stride)."""
-    if t.dtype != dtype or t.shape != shape or t.device != device:
-        raise ValueError(f"{name}: expected a {dtype} tensor of {tuple(shape)} on {device}, got {t.dtype} "
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != index:
+        raise ValueError(f"{name}: expected a {dtype} tensor of {tuple(shape)} on CUDA device {index}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     row, element = t.stride()
     if element != 1 and shape[1] > 1:
@@ -163,41 +163,41 @@ def rmsnorm(x, gamma=None, eps=1e-5, residual=None, sum_out=None, out=None, out_
     ([rows] f32) is given to receive them.  With neither ``out`` nor ``out_i8``, ``out`` is
     allocated.  Returns ``out`` if there is one, else ``out_i8``.
     """
-    dtype, shape, device = x.dtype, x.shape, x.device
+    dtype, shape, index = x.dtype, x.shape, x.get_device()
     code = _DTYPES.get(dtype)
-    if code is None or not x.is_cuda or len(shape) != 2:
-        raise ValueError(f"x: expected a 2-D CUDA f32, f16 or bf16 tensor, got {dtype} {tuple(shape)} on {device}")
-    px, sx = _rows(x, dtype, "x", shape, device)
+    if code is None or index < 0 or len(shape) != 2:
+        raise ValueError(f"x: expected a 2-D CUDA f32, f16 or bf16 tensor, got {dtype} {tuple(shape)} on {x.device}")
+    px, sx = _rows(x, dtype, "x", shape, index)
     if out is None and out_i8 is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = torch.empty(shape, dtype=dtype, device=x.device)
     rtype, rcode, pr, sr, ps, ss, po, so, pq, sq = dtype, code, None, 0, None, 0, None, 0, None, 0
     if residual is not None:
         rtype = residual.dtype
-        if rtype != dtype and rtype != torch.float32:
+        if rtype is not dtype and rtype is not torch.float32:
             raise ValueError(f"residual: expected {dtype} or f32, got {rtype}")
         rcode = _DTYPES[rtype]
-        pr, sr = _rows(residual, rtype, "residual", shape, device)
+        pr, sr = _rows(residual, rtype, "residual", shape, index)
     if sum_out is not None:
-        ps, ss = _rows(sum_out, rtype, "sum_out", shape, device)
+        ps, ss = _rows(sum_out, rtype, "sum_out", shape, index)
     if out is not None:
-        po, so = _rows(out, dtype, "out", shape, device)
+        po, so = _rows(out, dtype, "out", shape, index)
     if out_i8 is not None:
-        pq, sq = _rows(out_i8, torch.int8, "out_i8", shape, device)
+        pq, sq = _rows(out_i8, torch.int8, "out_i8", shape, index)
     for name, t, n in (("gamma", gamma, shape[1]), ("row_scales", row_scales, shape[0])):
-        if t is not None and (t.dtype != torch.float32 or t.numel() != n or t.device != device or
+        if t is not None and (t.dtype is not torch.float32 or t.numel() != n or t.get_device() != index or
                               not t.is_contiguous()):
-            raise ValueError(f"{name}: expected {n} contiguous f32 values on {device}, got {t.dtype} "
+            raise ValueError(f"{name}: expected {n} contiguous f32 values on {x.device}, got {t.dtype} "
                              f"{tuple(t.shape)} on {t.device}")
-    with _on(device):
+    with _on(index):
         check(lib().lsc_rmsnorm(px, code, sx, pr, rcode, sr, shape[0], shape[1],
                                 None if gamma is None else gamma.data_ptr(), eps, ps, ss, po, so, pq, sq, s_out,
-                                None if row_scales is None else row_scales.data_ptr(), rounding, _raw_stream(device)))
+                                None if row_scales is None else row_scales.data_ptr(), rounding, _raw_stream(index)))
     return out if out is not None else out_i8
 
 
-def _raw_stream(device):
-    """The current stream's handle as an int (torch's accessor without the Stream object)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _raw_stream(index):
+    """The current stream of device ``index``, as a handle (torch's accessor without the Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class _Here:
@@ -213,6 +213,6 @@ class _Here:
 _HERE = _Here()
 
 
-def _on(device):
-    """Makes ``device`` the current one for the call, as the library expects."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _on(index):
+    """Makes device ``index`` the current one for the call, as the library expects."""
+    return _HERE if torch._C._cuda_getDevice() == index else torch.cuda.device(index)

@@ -82,9 +82,20 @@ def test_prefill_refusals(kw):
     assert _prefill(_cache(), **kw) == _lib.ERROR_INVALID_ARGUMENT
 
 
-@pytest.mark.parametrize("kw", BOTH + [dict(ws=None), dict(ws=PTR + 8), dict(ws_bytes=0)])
+@pytest.mark.parametrize("kw", BOTH)
 def test_decode_refusals(kw):
     assert _decode(_cache(), **kw) == _lib.ERROR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("kw", [dict(ws=None), dict(ws=PTR + 8), dict(ws_bytes=0), dict(ws_bytes=1 << 20)])
+def test_decode_workspace_refusals(kw):
+    """A cache whose sequences can be cut needs a workspace; a short one needs none."""
+    long = _cache(max_pages=1000, table_stride=1000)
+    need = _lib.lib().lsc_paged_attention_decode_workspace_size(C.byref(long), 4)
+    assert need > 1 << 20
+    assert _decode(long, **kw) == _lib.ERROR_INVALID_ARGUMENT
+    assert "workspace" in _lib.last_error()
+    assert _lib.lib().lsc_paged_attention_decode_workspace_size(C.byref(_cache()), 4) == 0
 
 
 def test_empty_calls_succeed_without_a_device():
