@@ -246,11 +246,9 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
     // ------------------------------------------------------------------ TMA producer (whole warp)
     const int page_size = 1 << c.page_shift;
     const int box_rows = page_size < kTile ? page_size : kTile;
-    const int per_tile = kTile / box_rows;            // boxes of one column block
-    const int boxes = 2 * kBlocks * per_tile;         // of K and V: at most 32
+    const int per_tile = kTile / box_rows;  // boxes of K, and of V: at most 8
     const int sub = lane % per_tile;
-    const int block = (lane / per_tile) % kBlocks;
-    const bool is_v = lane / (per_tile * kBlocks) == 1;
+    const bool is_v = lane / per_tile == 1;
     uint32_t stage = 0, phase = 0;
     int issued = 0;
     bool ok = true;
@@ -275,10 +273,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
         if (!(ok = warp_wait(empty + stage, phase ^ 1u, abort_flag, c.err))) break;
         if (lane == 0) mbar_arrive_expect_tx(full + stage, 2 * Shape::kTileBytes);
         __syncwarp();
-        if (lane < boxes) {
+        if (lane < 2 * per_tile) {
           const int32_t j0 = cur.tiles.tile(i) * kTile + sub * box_rows;
-          uint8_t* dst = smem + (2 * stage + (is_v ? 1 : 0)) * Shape::kTileBytes + block * (kTile * 128) + sub * box_rows * 128;
-          tma_load_4d(is_v ? &tm_v : &tm_k, full + stage, dst, block * 64, j0 & (page_size - 1), kvh, page);
+          uint8_t* dst = smem + (2 * stage + (is_v ? 1 : 0)) * Shape::kTileBytes + sub * box_rows * (2 * D);
+          tma_load_5d(is_v ? &tm_v : &tm_k, full + stage, dst, 0, j0 & (page_size - 1), 0, kvh, page);
         }
         ++issued;
         if (++stage == kStages) {
@@ -304,6 +302,14 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
   // -------------------------------------------------------------------- multiplying warps
   const int slice = warp % kSlices, mt = warp / kSlices;
   const int r0 = lane >> 2, cpair = (lane & 3) * 2;
+  // A tile lies box by box (box_rows places), each box column block by column block: the bytes
+  // before place `key`, and between its column blocks
+  const int row_shift = c.page_shift < 6 ? c.page_shift : 6;
+  const uint32_t block_bytes = 128u << row_shift;
+  auto place = [&](int key) -> uint32_t {
+    return (static_cast<uint32_t>(key) >> row_shift) * (kBlocks * block_bytes) +
+           ((static_cast<uint32_t>(key) & ((1u << row_shift) - 1u)) << 7);
+  };
   uint32_t stage = 0, phase = 0, swap_phase = 0;
   int64_t at_tile = begin;
   if (!p.split && left < end - begin) at_tile = end - left;
@@ -349,11 +355,12 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
       for (int n = 0; n < kKeys / 16; ++n) {
         const int key = slice * kKeys + n * 16 + ((lane >> 4) << 3) + (lane & 7);
         const int half = (lane >> 3) & 1;
+        const uint32_t at = sk + place(key);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const int chunk = 2 * (k & 3) + half;
           uint32_t b[4];
-          ldsm4(sk + (k >> 2) * (kTile * 128) + key * 128 + ((chunk ^ (key & 7)) << 4), b);
+          ldsm4(at + (k >> 2) * block_bytes + ((chunk ^ (key & 7)) << 4), b);
           mma16816<BF16>(s[2 * n], q[k], b[0], b[1]);
           mma16816<BF16>(s[2 * n + 1], q[k], b[2], b[3]);
         }
@@ -413,11 +420,12 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
           keep1 = (keep(j + 8) ? 0xFFFFu : 0u) | (keep(j + 9) ? 0xFFFF0000u : 0u);
         }
         const int key = slice * kKeys + n * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+        const uint32_t at = sv + place(key);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const int chunk = 2 * (k & 3) + (lane >> 4);
           uint32_t b[4];
-          ldsm4_t(sv + (k >> 2) * (kTile * 128) + key * 128 + ((chunk ^ (key & 7)) << 4), b);
+          ldsm4_t(at + (k >> 2) * block_bytes + ((chunk ^ (key & 7)) << 4), b);
           mma16816<BF16>(o[2 * k], pa, b[0] & keep0, b[1] & keep1);
           mma16816<BF16>(o[2 * k + 1], pa, b[2] & keep0, b[3] & keep1);
         }
@@ -612,8 +620,8 @@ lsc_status launch_decode(const lsc_paged_kv* cache, const DeviceState* ds, const
   using Shape = DecodeShape<D>;
   const uint32_t box = cache->page_size < kTile ? cache->page_size : kTile;
   CUtensorMap tk, tv;
-  lsc_status s = paged_tensor_map(&tk, cache, c, cache->k, box);
-  if (s == LSC_SUCCESS) s = paged_tensor_map(&tv, cache, c, cache->v, box);
+  lsc_status s = paged_tensor_map(&tk, cache, c, cache->k, box, D / 64);
+  if (s == LSC_SUCCESS) s = paged_tensor_map(&tv, cache, c, cache->v, box, D / 64);
   if (s) return s;
   int grid = 2 * ds->sm_count;
   if (grid > kMaxCtas) grid = kMaxCtas;

@@ -29,9 +29,10 @@ lsc_status attention_args(const lsc_paged_kv* cache, const char* who, const void
                           int64_t q_token, int64_t q_head, float alpha, int64_t window, int64_t sinks, void* out,
                           int8_t* out_i8, float s_out, int32_t rounding, AttnArgs* a);
 
-// Tensor map of the keys or values {head_dim, page_size, heads, pages}, boxes of 64 x rows.
+// Tensor map of the keys or values {64, page_size, head_dim / 64, heads, pages}: boxes of box_rows
+// places x box_blocks column blocks of 64 elements, the blocks one after another in shared memory.
 lsc_status paged_tensor_map(CUtensorMap* map, const lsc_paged_kv* cache, const PagedView& view, const void* base,
-                            uint32_t box_rows);
+                            uint32_t box_rows, uint32_t box_blocks);
 
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;

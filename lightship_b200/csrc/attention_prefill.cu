@@ -150,42 +150,55 @@ struct Scheduler {
       top = other > top ? other : top;
     }
     total = at_or_above(0) * p.pairs;
+    level = top;
+    level_end = above = 0;
+    scan_b = scan_k = 0;
   }
-  // Unit number i (all lanes)
-  __device__ __forceinline__ Unit find(int64_t i) const {
+  // Unit number i (all lanes); calls come with growing i, so the level found and the place in the
+  // batch are kept: a large batch is scanned once per level.
+  int32_t level;               // of the unit before
+  int64_t level_end, above;    // F(level), F(level + 1)
+  int32_t scan_b, scan_k;      // first sequence of the block scanned last; units of the level before it
+  __device__ __forceinline__ Unit find(int64_t i) {
     const int64_t u = i / p.pairs;
     const int32_t pair = static_cast<int32_t>(i - u * p.pairs);
-    int32_t lo = 0, hi = top;  // F(lo) > u >= F(hi)
-    int64_t above = 0;         // F(hi)
-    while (hi - lo > 1) {
-      const int32_t mid = lo + (hi - lo) / 2;
-      const int64_t f = at_or_above(mid);
-      if (f > u) {
-        lo = mid;
-      } else {
-        hi = mid;
-        above = f;
+    if (u >= level_end) {
+      int32_t lo = 0, hi = level;  // F(lo) > u >= F(hi)
+      above = level_end;
+      level_end = total / p.pairs;
+      while (hi - lo > 1) {
+        const int32_t mid = lo + (hi - lo) / 2;
+        const int64_t f = at_or_above(mid);
+        if (f > u) {
+          lo = mid;
+          level_end = f;
+        } else {
+          hi = mid;
+          above = f;
+        }
       }
+      level = lo;
+      scan_b = scan_k = 0;
     }
-    // the (u - F(lo + 1))-th sequence with a unit at level lo
-    int32_t k = static_cast<int32_t>(u - above);
+    // the (u - above)-th sequence with a unit at this level
+    const int32_t k = static_cast<int32_t>(u - above);
     Unit r{};
 #pragma unroll 1
-    for (int b0 = 0; b0 < c.batch; b0 += 32) {
+    for (; scan_b < c.batch; scan_b += 32) {
       int32_t begin = 0, n = 0, base = 0, count = 0, len = 0;
-      if (b0 + lane < c.batch) of(b0 + lane, begin, n, base, count, len);
-      const bool here = base <= lo && lo < base + n;
+      if (scan_b + lane < c.batch) of(scan_b + lane, begin, n, base, count, len);
+      const bool here = base <= level && level < base + n;
       const uint32_t mask = __ballot_sync(0xffffffffu, here);
       const int have = __popc(mask);
-      if (k >= have) {
-        k -= have;
+      if (k >= scan_k + have) {
+        scan_k += have;
         continue;
       }
       uint32_t rest = mask;
-      for (; k > 0; --k) rest &= rest - 1;
+      for (int x = scan_k; x < k; ++x) rest &= rest - 1;
       const int src = __ffs(rest) - 1;
-      const int32_t first = (lo - base) * p.unit_tokens;
-      r.b = b0 + src;
+      const int32_t first = (level - base) * p.unit_tokens;
+      r.b = scan_b + src;
       r.row0 = __shfl_sync(0xffffffffu, begin + first, src);
       r.count = __shfl_sync(0xffffffffu, count - first < p.unit_tokens ? count - first : p.unit_tokens, src);
       r.pos0 = __shfl_sync(0xffffffffu, len - count + first, src);
@@ -293,7 +306,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           paged_len(c, b, true);
         }
       }
-      const Scheduler s(c, p, lane);
+      Scheduler s(c, p, lane);
       int64_t round = 0;         // of the next unit to find: the grid walks them to and fro
       int found = 0, zeroed = 0; // units passed on; units whose V rows are done
       bool more = true, ok = true;
@@ -379,7 +392,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const int page_size = 1 << c.page_shift;
       const int box_rows = page_size < kTile ? page_size : kTile;
       const int per_tile = kTile / box_rows;
-      const int boxes = per_tile * kBlocks;  // at most 32
+      // a box holds all column blocks where it has the whole tile's places, else one block
+      const int boxes = per_tile == 1 ? 1 : per_tile * kBlocks;  // at most 32
       const int sub = lane % per_tile, block = lane / per_tile;
       uint32_t stage0 = 0, phase0 = 0;  // of the unit's first K tile
       uint32_t land_parity = 0;         // per stage: uses of `landed` mod 2
@@ -414,9 +428,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           if (lane == 0) mbar_arrive_expect_tx(bar, Shape::kTileBytes);
           __syncwarp();
           if (lane < boxes)
-            tma_load_4d((x & 1) != 0 ? &tm_v : &tm_k, bar,
-                        s_kv + stage * Shape::kTileBytes + block * kBlockBytes + sub * box_rows * 128, block * 64,
-                        j0 & (page_size - 1), u.kvh, page);
+            tma_load_5d((x & 1) != 0 ? &tm_v : &tm_k, bar,
+                        s_kv + stage * Shape::kTileBytes + block * kBlockBytes + sub * box_rows * 128, 0,
+                        j0 & (page_size - 1), block, u.kvh, page);
           __syncwarp();
           used |= bit;
           if (by_landed) {
@@ -742,8 +756,9 @@ lsc_status launch_prefill(const lsc_paged_kv* cache, const DeviceState* ds, cons
   const AttnArgs& a = p.a;
   const uint32_t box = cache->page_size < kTile ? cache->page_size : kTile;
   CUtensorMap tq, tk, tv;
-  lsc_status s = paged_tensor_map(&tk, cache, c, cache->k, box);
-  if (s == LSC_SUCCESS) s = paged_tensor_map(&tv, cache, c, cache->v, box);
+  const uint32_t blocks = box == kTile ? D / 64 : 1;
+  lsc_status s = paged_tensor_map(&tk, cache, c, cache->k, box, blocks);
+  if (s == LSC_SUCCESS) s = paged_tensor_map(&tv, cache, c, cache->v, box, blocks);
   if (s) return s;
   const uint64_t dims[3] = {D, static_cast<uint64_t>(a.q_heads), static_cast<uint64_t>(a.tokens)};
   const uint64_t strides[2] = {static_cast<uint64_t>(a.q_head) * 2, static_cast<uint64_t>(a.q_token) * 2};
@@ -815,17 +830,18 @@ lsc_status attention_args(const lsc_paged_kv* cache, const char* who, const void
 }
 
 lsc_status paged_tensor_map(CUtensorMap* map, const lsc_paged_kv* cache, const PagedView& view, const void* base,
-                            uint32_t box_rows) {
-  const uint64_t dims[4] = {static_cast<uint64_t>(cache->head_dim), static_cast<uint64_t>(cache->page_size),
+                            uint32_t box_rows, uint32_t box_blocks) {
+  const uint64_t dims[5] = {64, static_cast<uint64_t>(cache->page_size), static_cast<uint64_t>(cache->head_dim / 64),
                             static_cast<uint64_t>(cache->kv_heads), static_cast<uint64_t>(cache->num_pages)};
-  const uint64_t strides[3] = {static_cast<uint64_t>(view.token_stride) * 2, static_cast<uint64_t>(view.head_stride) * 2,
-                               static_cast<uint64_t>(view.page_stride) * 2};
-  const uint32_t box[4] = {64, box_rows, 1, 1};
-  const uint32_t ones[4] = {1, 1, 1, 1};
-  return encode_tmap_4d(map, cache->dtype == LSC_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+  const uint64_t strides[4] = {static_cast<uint64_t>(view.token_stride) * 2, 128,
+                               static_cast<uint64_t>(view.head_stride) * 2, static_cast<uint64_t>(view.page_stride) * 2};
+  const uint32_t box[5] = {64, box_rows, box_blocks, 1, 1};
+  const uint32_t ones[5] = {1, 1, 1, 1, 1};
+  return encode_tmap_5d(map, cache->dtype == LSC_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                             : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                         base, dims, strides, box, ones, CU_TENSOR_MAP_SWIZZLE_128B);
 }
+
 }  // namespace lsc
 
 using namespace lsc;

@@ -78,6 +78,10 @@ lsc_status encode_tmap_4d(CUtensorMap* map, CUtensorMapDataType dtype, const voi
                           const uint64_t dims[4], const uint64_t strides_bytes[3],
                           const uint32_t box[4], const uint32_t elem_strides[4],
                           CUtensorMapSwizzle swizzle);
+lsc_status encode_tmap_5d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base,
+                          const uint64_t dims[5], const uint64_t strides_bytes[4],
+                          const uint32_t box[5], const uint32_t elem_strides[5],
+                          CUtensorMapSwizzle swizzle);
 
 // 4-D NHWC tensor map in im2col mode (cuTensorMapEncodeIm2col).
 lsc_status encode_tmap_im2col(CUtensorMap* map, CUtensorMapDataType dtype, const void* base,

@@ -198,6 +198,17 @@ lsc_status encode_tmap_4d(CUtensorMap* map, CUtensorMapDataType dtype, const voi
   return encode(map, dtype, 4, base, d, s, b, e, swizzle);
 }
 
+lsc_status encode_tmap_5d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base,
+                          const uint64_t dims[5], const uint64_t strides_bytes[4],
+                          const uint32_t box[5], const uint32_t elem_strides[5],
+                          CUtensorMapSwizzle swizzle) {
+  const cuuint64_t d[5] = {dims[0], dims[1], dims[2], dims[3], dims[4]};
+  const cuuint64_t s[4] = {strides_bytes[0], strides_bytes[1], strides_bytes[2], strides_bytes[3]};
+  const cuuint32_t b[5] = {box[0], box[1], box[2], box[3], box[4]};
+  const cuuint32_t e[5] = {elem_strides[0], elem_strides[1], elem_strides[2], elem_strides[3], elem_strides[4]};
+  return encode(map, dtype, 5, base, d, s, b, e, swizzle);
+}
+
 }  // namespace lsc
 
 using namespace lsc;
