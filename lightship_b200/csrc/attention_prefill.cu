@@ -34,7 +34,8 @@ namespace {
 constexpr int kTile = 128;            // rows of a row tile, places of a key tile
 constexpr int kPrefillThreads = 384;
 constexpr int kSchedSlots = 4;
-constexpr int kParts = 2;              // parts of P that are passed on, of 64 keys each
+constexpr int kParts = 2;              // parts of P that are passed on
+constexpr int kFirstPart = 96;         // keys of the first (the products of the last are waited for)
 constexpr int kTurnAt = 3;             // the quarter of the exponentials after which the other row tile may begin
 constexpr float kMoveBy = 8.0f;       // log2 of how far a maximum may pass the reference
 
@@ -538,9 +539,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           for (int32_t x = i + 1; x < j; ++x) step(ks, kph, 2);
           const uint64_t dka = dk + ks * kDescTile;
           auto products = [&](auto part) {  // by the elected lane
-            constexpr int kSteps = kTile / 16 / kParts, x = decltype(part)::value;
+            constexpr int x = decltype(part)::value, kCut = kFirstPart / 16;
 #pragma unroll
-            for (int k = x * kSteps; k < (x + 1) * kSteps; ++k)
+            for (int k = x ? kCut : 0; k < (x ? kTile / 16 : kCut); ++k)
               mma_f16_ts(t_o, t_s + k * 8, dva + k * (2048 >> 4), idesc_o, k != 0 ? 1u : more);
           };
           if (!(ok = warp_wait(p_full + w * kParts, p_phase, abort_flag, c.err))) break;
@@ -683,7 +684,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             packed[e] = pack16<BF16>(y0, y1);
           }
           if (shared && x == kTurnAt && lane == 0) mbar_arrive(turn + (w ^ 1));
-          if (x == 2) arrive(0);  // its stores have had the time of 32 keys to complete
+          if (x == kFirstPart / 32) arrive(0);  // its stores have had the time of 32 keys to complete
           tmem_st_32x32b_x16(t_s + 16 * x, packed);
         }
         arrive(1);
