@@ -52,7 +52,14 @@ struct PrefillShape {
   static constexpr int kStages = D == 128 ? 5 : 10;   // K and V tiles in turn
   static constexpr int kBarBytes = 768;
   static constexpr int kSmem = (2 + kStages) * kTileBytes + kBarBytes + 1024;
-  static constexpr uint32_t kColS = 0, kColO = 256;   // TMEM columns: S of both tiles, then O of both
+  // TMEM columns of a row tile's S and P, then O of both.  Heads of 128 leave 128 columns for S, and P
+  // takes its place: the next S waits for the products with P.  Heads of 64 leave 192 (kApart): tiles
+  // take turns at S in the last or the first 128 and P in the last or the first 64 of them, so the next
+  // S never meets the P in use and is there when the softmax comes for it.
+  static constexpr bool kApart = D == 64;
+  static constexpr uint32_t kColsS = kApart ? 192 : 128, kColO = 2 * kColsS;
+  static constexpr uint32_t s_at(uint32_t turn) { return kApart && turn == 0 ? 64 : 0; }
+  static constexpr uint32_t p_at(uint32_t turn) { return kApart && turn == 0 ? 128 : 0; }
 };
 static_assert(PrefillShape<128>::kSmem <= 232448 && PrefillShape<64>::kSmem <= 232448, "shared memory budget");
 
@@ -231,8 +238,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   uint64_t* q_full = landed + kStages;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;
-  uint64_t* p_full = s_full + 2;  // [row tile][part]
-  uint64_t* o_full = p_full + 2 * kParts;
+  uint64_t* p_full = s_full + 2;  // [row tile][turn][part]
+  uint64_t* o_last = p_full + 4 * kParts;  // (kApart) the product before a unit's last one is complete
+  uint64_t* s_free = o_last + 2;           // (kApart) the softmax has S in registers
+  uint64_t* o_full = s_free + 2;
   uint64_t* drain = o_full + 2;
   uint64_t* turn = drain + 2;  // [row tile]: the other one has done its exponentials
   uint64_t* sched_full = turn + 2;
@@ -253,7 +262,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     mbar_init(q_empty, 2);
     for (int w = 0; w < 2; ++w) {
       mbar_init(s_full + w, 1);
-      for (int x = 0; x < kParts; ++x) mbar_init(p_full + w * kParts + x, 4);
+      for (int x = 0; x < 2 * kParts; ++x) mbar_init(p_full + 2 * w * kParts + x, 4);
+      mbar_init(o_last + w, 1);
+      mbar_init(s_free + w, 4);
       mbar_init(o_full + w, 1);
     }
     for (int w = 0; w < 2; ++w) {
@@ -469,8 +480,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const uint64_t dq = smem_desc_sw128_kmajor(smem_u32(s_q + w * Shape::kTileBytes));
       const uint64_t dk = smem_desc_sw128_kmajor(smem_u32(s_kv));
       const uint64_t dv = smem_desc_sw128_mnmajor(smem_u32(s_kv), kBlockBytes);
-      const uint32_t t_s = uniform(tmem) + Shape::kColS + w * kTile, t_o = uniform(tmem) + Shape::kColO + w * D;
-      uint32_t q_phase = 0, p_phase = 0;
+      const uint32_t t_s = uniform(tmem) + w * Shape::kColsS, t_o = uniform(tmem) + Shape::kColO + w * D;
+      uint32_t q_phase = 0, p_phase = 0, free_phase = 0;  // p_phase: a bit per turn
       uint32_t stage = 0, phase = 0;  // of the next K tile that has not been used
       bool ok = true, any = false;
       auto step = [](uint32_t& s, uint32_t& ph, uint32_t by) {
@@ -480,13 +491,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           ph ^= 1u;
         }
       };
-      // One commit per key tile, behind its scores.  The softmax warps, which wait for it, give back the
-      // stages that it shows to be free.
-      auto issue_scores = [&](uint64_t dka) {  // by the elected lane
+      // A commit holds up the issuing lane for about as long as three products, so there is one per key
+      // tile, behind its scores.  The softmax warps, which wait for it, give back the stages that it
+      // shows to be free.
+      auto issue_scores = [&](uint32_t turn_of, uint64_t dka) {  // by the elected lane
+        const uint32_t to = t_s + (turn_of == 0 ? Shape::s_at(0) : Shape::s_at(1));
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           constexpr int kStep = 32 >> 4, kBlock = kBlockBytes >> 4;
-          mma_f16(t_s, dq + (k >> 2) * kBlock + (k & 3) * kStep, dka + (k >> 2) * kBlock + (k & 3) * kStep, idesc_s,
+          mma_f16(to, dq + (k >> 2) * kBlock + (k & 3) * kStep, dka + (k >> 2) * kBlock + (k & 3) * kStep, idesc_s,
                   k != 0 ? 1u : 0u);
         }
         mma_commit(s_full + w);
@@ -510,19 +523,21 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           for (int32_t i = 0; i < first; ++i) step(s, ph, 2);
           if (!(ok = warp_wait(kv_full + s, ph, abort_flag, c.err))) break;
           tc_fence_after();
-          if (elect_one()) issue_scores(dk + s * kDescTile);
+          if (elect_one()) issue_scores(0, dk + s * kDescTile);
           __syncwarp();
           any = true;
         } else {
           if (lane == 0) mbar_arrive(q_empty);  // no softmax warp will
           __syncwarp();
         }
+        uint32_t turn_of = 0;  // of the row tile's tiles, every other
         for (int32_t i = 0; i < n; ++i) {
           uint32_t vs = stage, vph = phase, ks = stage, kph = phase;
           step(vs, vph, 1);
           step(ks, kph, 2);
-          if (!(ok = warp_wait(kv_full + vs, vph, abort_flag, c.err))) break;
-          if (!span.has(i)) {
+          const bool mine = span.has(i);
+          if ((!Shape::kApart || !mine) && !(ok = warp_wait(kv_full + vs, vph, abort_flag, c.err))) break;
+          if (!mine) {
             // Not this row tile's: give the stages back once they hold the tile (before, the arrival
             // would count for the tile that they held last).
             if (!(ok = warp_wait(kv_full + stage, phase, abort_flag, c.err))) break;
@@ -538,27 +553,44 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           const int32_t j = span.next(i);
           for (int32_t x = i + 1; x < j; ++x) step(ks, kph, 2);
           const uint64_t dka = dk + ks * kDescTile;
+          const uint32_t t_p = t_s + (turn_of == 0 ? Shape::p_at(0) : Shape::p_at(1));
           auto products = [&](auto part) {  // by the elected lane
             constexpr int x = decltype(part)::value, kCut = kFirstPart / 16;
 #pragma unroll
             for (int k = x ? kCut : 0; k < (x ? kTile / 16 : kCut); ++k)
-              mma_f16_ts(t_o, t_s + k * 8, dva + k * (2048 >> 4), idesc_o, k != 0 ? 1u : more);
+              mma_f16_ts(t_o, t_p + k * 8, dva + k * (2048 >> 4), idesc_o, k != 0 ? 1u : more);
           };
-          if (!(ok = warp_wait(p_full + w * kParts, p_phase, abort_flag, c.err))) break;
+          if constexpr (Shape::kApart) {
+            if (j < n) {
+              if (!(ok = warp_wait(kv_full + ks, kph, abort_flag, c.err))) break;
+              if (!(ok = warp_wait(s_free + w, free_phase, abort_flag, c.err))) break;
+              free_phase ^= 1u;
+              tc_fence_after();
+              if (elect_one()) issue_scores(turn_of ^ 1u, dka);
+              __syncwarp();
+            }
+            if (!(ok = warp_wait(kv_full + vs, vph, abort_flag, c.err))) break;
+          }
+          uint64_t* const p_ready = p_full + (2 * w + (Shape::kApart ? turn_of : 0)) * kParts;
+          const uint32_t p_parity = (p_phase >> (Shape::kApart ? turn_of : 0)) & 1u;
+          if (!(ok = warp_wait(p_ready, p_parity, abort_flag, c.err))) break;
           tc_fence_after();
           if (elect_one()) products(std::integral_constant<int, 0>{});
           __syncwarp();
-          if (j < n && !(ok = warp_wait(kv_full + ks, kph, abort_flag, c.err))) break;
-          if (!(ok = warp_wait(p_full + w * kParts + 1, p_phase, abort_flag, c.err))) break;
+          if (!Shape::kApart && j < n && !(ok = warp_wait(kv_full + ks, kph, abort_flag, c.err))) break;
+          if (!(ok = warp_wait(p_ready + 1, p_parity, abort_flag, c.err))) break;
           tc_fence_after();
           if (elect_one()) {
             products(std::integral_constant<int, 1>{});
-            // S of the row tile's next tile follows its products into O, which read P in S's place
-            if (j < n) issue_scores(dka);
-            else mma_commit(o_full + w);
+            // heads of 128: S of the row tile's next tile follows its products into O, which read P in S's
+            // place; heads of 64: it was issued before
+            if (j >= n) mma_commit(o_full + w);
+            else if (!Shape::kApart) issue_scores(0, dka);
+            else if (span.next(j) >= n) mma_commit(o_last + w);
           }
           __syncwarp();
-          p_phase ^= 1u;
+          p_phase ^= Shape::kApart ? 1u << turn_of : 1u;
+          turn_of ^= Shape::kApart ? 1u : 0u;
           more = 1;
           step(stage, phase, 2);
         }
@@ -578,11 +610,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     const int w = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t t_s = tmem + lanes + Shape::kColS + w * kTile;
+    const uint32_t t_s = tmem + lanes + w * Shape::kColsS;
     const uint32_t t_o = tmem + lanes + Shape::kColO + w * D;
     const int token = row / p.hp, head = row - token * p.hp;
     const float scale = a.scale_log2;
-    uint32_t s_phase = 0, o_phase = 0;
+    uint32_t s_phase = 0, o_phase = 0, last_phase = 0;
     uint32_t stage0 = 0;  // of the unit's first K tile
     uint32_t turn_phase = w == 0 ? 1u : 0u;  // row tile 0 begins
     Unit u;
@@ -606,16 +638,26 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       float ref = -INFINITY;  // the reference m, in units of the raw scores
       float l = 0.0f;
       int done = 0;
-      int32_t before = -1;  // the tile before i
-      for (int32_t i = span.next(-1); i < tiles.n; i = span.next(i)) {
-        const int32_t j0 = tiles.tile(i) * kTile;
+      int32_t before = -1, before2 = -1;  // the tile before i, and the one before that
+      for (int32_t i = span.next(-1); i < tiles.n;) {
+        const int32_t j0 = tiles.tile(i) * kTile, after = span.next(i);
+        const uint32_t turn_of = Shape::kApart ? done & 1u : 0u;
+        const uint32_t s_here = t_s + (turn_of == 0 ? Shape::s_at(0) : Shape::s_at(1));
+        const uint32_t p_here = t_s + (turn_of == 0 ? Shape::p_at(0) : Shape::p_at(1));
         if (!(ok = warp_wait(s_full + w, s_phase, abort_flag, c.err))) break;
         s_phase ^= 1u;
         tc_fence_after();
+        // the unit's last scores are there: Q of the next one may come
+        if (after >= tiles.n && quarter == 0 && lane == 0) mbar_arrive(q_empty);
         uint32_t s[4][32];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) tmem_ld_32x32b_x32(t_s + 32 * x, s[x]);
+        for (int x = 0; x < 4; ++x) tmem_ld_32x32b_x32(s_here + 32 * x, s[x]);
         tmem_ld_wait();
+        if constexpr (Shape::kApart) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0 && after < tiles.n) mbar_arrive(s_free + w);
+        }
         if (j0 + kTile - 1 > pos_min || (j0 < low_max && j0 + kTile > a.sinks)) {
           // some row of the warp does not see the whole tile: -inf in the places it does not see
 #pragma unroll
@@ -640,6 +682,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           // also true where ref is -inf and m is not; false where both are
           const bool move = (m - ref) * scale > kMoveBy;
           if (__any_sync(0xffffffffu, move)) {
+            if constexpr (Shape::kApart) {
+              // The product of the tile before is complete when the next tile's scores, issued behind it,
+              // are; where no scores follow it has a barrier of its own.
+              if (after < tiles.n) ok = warp_wait(s_full + w, s_phase, abort_flag, c.err);
+              else ok = warp_wait(o_last + w, last_phase, abort_flag, c.err);
+              if (!ok) break;
+              tc_fence_after();
+            }
             const float f = move ? ex2_approx((ref - m) * scale) : 1.0f;
             if (move) ref = m;
             l *= f;
@@ -654,7 +704,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             }
           }
         }
-        done = 1;
+        ++done;
         const float shift = ref == -INFINITY ? 0.0f : -ref * scale;
         const uint64_t scale2 = f2pack(scale, scale), shift2 = f2pack(shift, shift);
         uint64_t sum2[2] = {0ull, 0ull};
@@ -669,7 +719,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(p_full + w * kParts + part);
+          if (lane == 0) mbar_arrive(p_full + (2 * w + turn_of) * kParts + part);
         };
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
@@ -685,26 +735,32 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           }
           if (shared && x == kTurnAt && lane == 0) mbar_arrive(turn + (w ^ 1));
           if (x == kFirstPart / 32) arrive(0);  // its stores have had the time of 32 keys to complete
-          tmem_st_32x32b_x16(t_s + 16 * x, packed);
+          tmem_st_32x32b_x16(p_here + 16 * x, packed);
         }
         arrive(1);
         if (quarter == 0 && lane == 0) {
           // with the scores all products issued before them were complete
           release(i, 0);
-          if (before >= 0) release(before, 1);
-          if (span.next(i) >= tiles.n) mbar_arrive(q_empty);
+          const int32_t past = Shape::kApart ? before2 : before;
+          if (past >= 0) release(past, 1);
         }
+        before2 = before;
         before = i;
         float s0, s1;
         f2unpack(f2add(sum2[0], sum2[1]), s0, s1);
         l += s0 + s1;
+        i = after;
       }
       if (!ok) break;
       if (done) {
         if (!(ok = warp_wait(o_full + w, o_phase, abort_flag, c.err))) break;
         o_phase ^= 1u;
         tc_fence_after();
-        if (quarter == 0 && lane == 0) release(before, 1);
+        if (quarter == 0 && lane == 0) {
+          release(before, 1);
+          if (Shape::kApart && before2 >= 0) release(before2, 1);
+        }
+        if (done >= 2) last_phase ^= 1u;
       }
       const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
       const int64_t at = (static_cast<int64_t>(u.row0 + w * p.tpt + token) * a.q_heads + u.head0 + head) * D;
