@@ -122,23 +122,30 @@ struct Scheduler {
   int lane;
   int64_t total;
   int32_t top;
-  __device__ __forceinline__ void of(int b, int32_t& begin, int32_t& n, int32_t& base, int32_t& count,
-                                     int32_t& len) const {
+  // What is known of sequence b: its rows, its length, its units and their first level.
+  struct Seq {
+    int32_t begin, count, len, n, base;
+  };
+  Seq held;  // of sequence `lane`: batches of up to 32 are read once
+  __device__ __forceinline__ Seq read(int b) const {
+    Seq s{};
+    if (b >= c.batch) return s;
     int32_t end;
-    query_rows(p.a.offsets, b, p.a.tokens, c.err, false, begin, end);
-    len = paged_len(c, b, false);
-    count = end - begin;
-    n = (count + p.unit_tokens - 1) / p.unit_tokens;
-    base = len > count ? (len - count) / p.unit_tokens : 0;
+    query_rows(p.a.offsets, b, p.a.tokens, c.err, false, s.begin, end);
+    s.len = paged_len(c, b, false);
+    s.count = end - s.begin;
+    s.n = (s.count + p.unit_tokens - 1) / p.unit_tokens;
+    s.base = s.len > s.count ? (s.len - s.count) / p.unit_tokens : 0;
+    return s;
   }
+  __device__ __forceinline__ Seq of(int b) const { return b == lane ? held : read(b); }
   __device__ __forceinline__ int64_t at_or_above(int32_t t) const {
     int64_t f = 0;
 #pragma unroll 1
     for (int b = lane; b < c.batch; b += 32) {
-      int32_t begin, n, base, count, len;
-      of(b, begin, n, base, count, len);
-      const int32_t x = base + n - t;
-      f += x < 0 ? 0 : (x > n ? n : x);
+      const Seq s = of(b);
+      const int32_t x = s.base + s.n - t;
+      f += x < 0 ? 0 : (x > s.n ? s.n : x);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) f += __shfl_xor_sync(0xffffffffu, f, o);
@@ -146,11 +153,11 @@ struct Scheduler {
   }
   __device__ __forceinline__ Scheduler(const PagedView& c_, const PrefillArgs& p_, int lane_)
       : c(c_), p(p_), lane(lane_), top(0) {
+    held = read(lane);
 #pragma unroll 1
     for (int b = lane; b < c.batch; b += 32) {
-      int32_t begin, n, base, count, len;
-      of(b, begin, n, base, count, len);
-      top = n > 0 && base + n > top ? base + n : top;
+      const Seq s = of(b);
+      top = s.n > 0 && s.base + s.n > top ? s.base + s.n : top;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -193,9 +200,8 @@ struct Scheduler {
     Unit r{};
 #pragma unroll 1
     for (; scan_b < c.batch; scan_b += 32) {
-      int32_t begin = 0, n = 0, base = 0, count = 0, len = 0;
-      if (scan_b + lane < c.batch) of(scan_b + lane, begin, n, base, count, len);
-      const bool here = base <= level && level < base + n;
+      const Seq s = of(scan_b + lane);
+      const bool here = s.base <= level && level < s.base + s.n;
       const uint32_t mask = __ballot_sync(0xffffffffu, here);
       const int have = __popc(mask);
       if (k >= scan_k + have) {
@@ -205,11 +211,11 @@ struct Scheduler {
       uint32_t rest = mask;
       for (int x = scan_k; x < k; ++x) rest &= rest - 1;
       const int src = __ffs(rest) - 1;
-      const int32_t first = (level - base) * p.unit_tokens;
+      const int32_t first = (level - s.base) * p.unit_tokens;
       r.b = scan_b + src;
-      r.row0 = __shfl_sync(0xffffffffu, begin + first, src);
-      r.count = __shfl_sync(0xffffffffu, count - first < p.unit_tokens ? count - first : p.unit_tokens, src);
-      r.pos0 = __shfl_sync(0xffffffffu, len - count + first, src);
+      r.row0 = __shfl_sync(0xffffffffu, s.begin + first, src);
+      r.count = __shfl_sync(0xffffffffu, s.count - first < p.unit_tokens ? s.count - first : p.unit_tokens, src);
+      r.pos0 = __shfl_sync(0xffffffffu, s.len - s.count + first, src);
       break;
     }
     const int32_t per_head = p.pairs / c.kv_heads;
@@ -324,7 +330,25 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       bool more = true, ok = true;
       uint32_t stage = 0, land_phase = 0;  // land_phase: one parity bit per stage
       uint32_t q_phase = 0;
-      int q_loads = 0;
+      int q_loads = 0, q_units = 0;  // copies; units whose Q is on its way (or not needed)
+      // Q of a unit, once the scores of the unit before are done (they need no more from this warp)
+      auto bring_q = [&](const Unit& u) -> bool {
+        ++q_units;
+        if (tiles_of(u).n == 0) return true;
+        if (!warp_wait(q_empty, q_phase ^ 1u, abort_flag, c.err)) return false;
+        q_phase ^= 1u;
+        if (lane == 0) {
+          const int q_tiles = u.count > p.tpt ? 2 : 1;
+          mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(q_tiles * kBlocks * p.hp * p.tpt * 128));
+          for (int w = 0; w < q_tiles; ++w)
+            for (int x = 0; x < kBlocks; ++x)
+              tma_load_3d(&tm_q, q_full, s_q + w * Shape::kTileBytes + x * kBlockBytes, x * 64, u.head0,
+                          u.row0 + w * p.tpt);
+        }
+        __syncwarp();
+        ++q_loads;
+        return true;
+      };
       while (ok && (more || zeroed < found)) {
         // Pass on the next unit as soon as its slot is free, but wait for a slot only when there is
         // nothing to zero: the others need no more from this warp to free one.
@@ -350,25 +374,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             sched_phase ^= 1u;
           }
           if (more) ++found;
+          // the first unit's Q comes before the others are looked for
+          if (more && q_units == 0 && !(ok = bring_q(u))) break;
           continue;
         }
         const Unit u = sched[zeroed % kSchedSlots];
-        ++zeroed;
         const TileList<kTile> tiles = tiles_of(u);
+        if (q_units == zeroed && !(ok = bring_q(u))) break;
+        ++zeroed;
         if (tiles.n == 0) continue;
-        // Q, once the scores of the unit before are done (they need no more from this warp)
-        if (!(ok = warp_wait(q_empty, q_phase ^ 1u, abort_flag, c.err))) break;
-        q_phase ^= 1u;
-        if (lane == 0) {
-          const int q_tiles = u.count > p.tpt ? 2 : 1;
-          mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(q_tiles * kBlocks * p.hp * p.tpt * 128));
-          for (int w = 0; w < q_tiles; ++w)
-            for (int x = 0; x < kBlocks; ++x)
-              tma_load_3d(&tm_q, q_full, s_q + w * Shape::kTileBytes + x * kBlockBytes, x * 64, u.head0,
-                          u.row0 + w * p.tpt);
-        }
-        __syncwarp();
-        ++q_loads;
         const int32_t last = u.pos0 + u.count - 1;
         const int32_t low = a.window > 0 && u.pos0 >= a.window ? u.pos0 - a.window + 1 : 0;
         for (int32_t i = 0; i < tiles.n; ++i) {
