@@ -475,7 +475,7 @@ typedef struct lsc_paged_kv {
 
 /* Writes the new tokens' keys and values into their pages.  Sequence b's new tokens are rows
  * q_offsets[b] .. q_offsets[b + 1] - 1 of k_new / v_new (device int32 [batch + 1]; `tokens` rows
- * in all) and take its last places, up to kv_lens[b] - 1; a new token that would come before
+ * in all, at most 2^30) and take its last places, up to kv_lens[b] - 1; a new token that would come before
  * place 0 is left out and raises the error word.  Rows before the first offset or behind the
  * last one are not read.  Row t, head h is at k_new + t * new_token_stride + h * new_head_stride
  * (elements, multiples of 8; 16-byte aligned bases): the K and V parts of a fused QKV projection

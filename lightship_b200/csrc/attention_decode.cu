@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
         const int32_t j0 = cur.tiles.tile(i) * kTile + sub * box_rows;
         const bool seen = j0 < cur.len && (j0 + box_rows > low || j0 < a.sinks);
         if (!seen) return static_cast<int32_t>(c.num_pages);
-        const int32_t id = __ldg(c.table + cur.b * c.table_stride + (j0 >> c.page_shift));
+        const int32_t id = *(c.table + cur.b * c.table_stride + (j0 >> c.page_shift));
         if (id >= 0 && id < c.num_pages) return id;
         raise_bad_arg(c.err);
         return static_cast<int32_t>(c.num_pages);
@@ -330,10 +330,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
       const uint16_t* qb = base + rb * a.q_head;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        q[k][0] = ra < heads ? __ldg(reinterpret_cast<const uint32_t*>(qa + 16 * k)) : 0u;
-        q[k][1] = rb < heads ? __ldg(reinterpret_cast<const uint32_t*>(qb + 16 * k)) : 0u;
-        q[k][2] = ra < heads ? __ldg(reinterpret_cast<const uint32_t*>(qa + 16 * k + 8)) : 0u;
-        q[k][3] = rb < heads ? __ldg(reinterpret_cast<const uint32_t*>(qb + 16 * k + 8)) : 0u;
+        q[k][0] = ra < heads ? *reinterpret_cast<const uint32_t*>(qa + 16 * k) : 0u;
+        q[k][1] = rb < heads ? *reinterpret_cast<const uint32_t*>(qb + 16 * k) : 0u;
+        q[k][2] = ra < heads ? *reinterpret_cast<const uint32_t*>(qa + 16 * k + 8) : 0u;
+        q[k][3] = rb < heads ? *reinterpret_cast<const uint32_t*>(qb + 16 * k + 8) : 0u;
       }
     }
     float o[D / 8][4];
@@ -550,8 +550,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
   }
 }
 
-// Joins the parts of the pair that CTA blockIdx.x opened and did not close, for row blockIdx.y:
-// eight warps take every eighth part, in the order of the CTAs.
+// Joins the parts of the pair that CTA blockIdx.x opened and did not close, for rows blockIdx.y,
+// blockIdx.y + gridDim.y, ...: eight warps take every eighth part, in the order of the CTAs.
 template <bool BF16, int D, int MT>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedView c, const DecodeArgs p, int grid) {
   constexpr int kRows = 16 * MT, kVec = D / 32;
@@ -559,45 +559,49 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedView c, cons
   __shared__ float acc_l[8];
   griddep_wait();
   griddep_launch_dependents();
-  const int cta = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int32_t parts = p.desc[4 * cta + 2];
   if (parts == 0) return;
   const int32_t b = p.desc[4 * cta], pair = p.desc[4 * cta + 1];
-  const int kvh = pair / p.head_tiles, head = (pair - kvh * p.head_tiles) * kRows + row;
-  if (head >= p.a.group) return;
-  // part x lies in the opening slot (x = 0) or in the first-segment slot of CTA cta + x
-  auto slot = [&](int x) { return static_cast<int64_t>(x == 0 ? grid + cta : cta + x) * kRows + row; };
-  float top = -INFINITY;
-  for (int x = lane; x < parts; x += 32) top = fmaxf(top, p.part_m[slot(x)]);
+  const int kvh = pair / p.head_tiles, head0 = (pair - kvh * p.head_tiles) * kRows;
+  for (int row = blockIdx.y; row < kRows && head0 + row < p.a.group; row += gridDim.y) {
+    const int head = head0 + row;
+    // part x lies in the opening slot (x = 0) or in the first-segment slot of CTA cta + x
+    auto slot = [&](int x) { return static_cast<int64_t>(x == 0 ? grid + cta : cta + x) * kRows + row; };
+    float top = -INFINITY;
+    for (int x = lane; x < parts; x += 32) top = fmaxf(top, p.part_m[slot(x)]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float ref = top == -INFINITY ? 0.0f : top;
-  float v[kVec] = {}, l = 0.0f;
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float v[kVec] = {}, l = 0.0f;
 #pragma unroll 4
-  for (int x = warp; x < parts; x += 8) {
-    const int64_t s = slot(x);
-    const float f = ex2_approx(p.part_m[s] - ref);
-    l += f * p.part_l[s];
-    const float* from = p.part_o + s * D + lane * kVec;
+    for (int x = warp; x < parts; x += 8) {
+      const int64_t s = slot(x);
+      const float f = ex2_approx(p.part_m[s] - ref);
+      l += f * p.part_l[s];
+      const float* from = p.part_o + s * D + lane * kVec;
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) v[e] += f * from[e];
+      for (int e = 0; e < kVec; ++e) v[e] += f * from[e];
+    }
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) acc[warp][lane * kVec + e] = v[e];
+    if (lane == 0) acc_l[warp] = l;
+    __syncthreads();
+    const int d = threadIdx.x * 2;
+    if (d < D) {
+      float x = 0.0f, y = 0.0f;
+      l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        x += acc[w][d];
+        y += acc[w][d + 1];
+        l += acc_l[w];
+      }
+      const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
+      write_pair<BF16>(p.a, (static_cast<int64_t>(b) * p.a.q_heads + kvh * p.a.group + head) * D + d, x * inv, y * inv);
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) acc[warp][lane * kVec + e] = v[e];
-  if (lane == 0) acc_l[warp] = l;
-  __syncthreads();
-  const int d = threadIdx.x * 2;
-  if (d >= D) return;
-  float x = 0.0f, y = 0.0f;
-  l = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    x += acc[w][d];
-    y += acc[w][d + 1];
-    l += acc_l[w];
-  }
-  const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
-  write_pair<BF16>(p.a, (static_cast<int64_t>(b) * p.a.q_heads + kvh * p.a.group + head) * D + d, x * inv, y * inv);
 }
 
 // Row tiles of a group: 16 heads while they suffice, then 32, then 64 (and several of those).
@@ -630,7 +634,7 @@ lsc_status launch_decode(const lsc_paged_kv* cache, const DeviceState* ds, const
   LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, paged_decode_kernel<BF16, D, MT>, dim3(grid),
                                 dim3(kDecodeThreads), Shape::kSmem, st, tk, tv, c, p));
   if (p.split) {
-    const int rows = p.a.group < 16 * MT ? p.a.group : 16 * MT;
+    const int rows = p.a.group < 16 ? p.a.group : 16;
     LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, paged_join_kernel<BF16, D, MT>, dim3(grid, rows), dim3(256), 0,
                                   st, c, p, grid));
   }

@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         auto page_of = [&](int32_t i) -> int32_t {
           const int32_t j0 = tiles.tile(i) * kTile + sub * box_rows;
           const bool seen = j0 <= last && (j0 + box_rows > low || j0 < a.sinks);
-          return seen ? __ldg(c.table + u.b * c.table_stride + (j0 >> c.page_shift)) : kUnseen;
+          return seen ? c.table[u.b * c.table_stride + (j0 >> c.page_shift)] : kUnseen;
         };
         const int32_t count = 2 * tiles.n;  // K tiles even, V tiles odd
         int32_t next = page_of(0);
@@ -859,7 +859,8 @@ lsc_status launch_prefill(const lsc_paged_kv* cache, const DeviceState* ds, cons
 lsc_status attention_args(const lsc_paged_kv* cache, const char* who, const void* q, int64_t tokens, int32_t q_heads,
                           int64_t q_token, int64_t q_head, float alpha, int64_t window, int64_t sinks, void* out,
                           int8_t* out_i8, float s_out, int32_t rounding, AttnArgs* a) {
-  if (tokens < 0 || tokens > INT32_MAX) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: bad token count", who);
+  if (tokens < 0 || tokens > (1 << 30))
+    return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: bad token count (at most 2^30)", who);
   if (q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads)
     return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: %d query heads are not a multiple of %d key-value heads", who,
                      q_heads, cache->kv_heads);
@@ -931,7 +932,8 @@ extern "C" lsc_status lsc_paged_attention_prefill(const lsc_paged_kv* cache, con
                       s_out, rounding, &p.a);
   if (st) return st;
   if (tokens == 0 || c.batch == 0) return LSC_SUCCESS;
-  if (!q_offsets) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: null offsets", who);
+  if (!q_offsets || (reinterpret_cast<uintptr_t>(q_offsets) & 3))
+    return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: null or misaligned offsets", who);
   p.a.offsets = q_offsets;
   DeviceState* ds = nullptr;
   if ((st = paged_device(who, &ds, &c))) return st;

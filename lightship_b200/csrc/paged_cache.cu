@@ -22,6 +22,8 @@ lsc_status paged_view(const lsc_paged_kv* c, const char* who, PagedView* view) {
     return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: bad page counts (at most 2^30 places per sequence)", who);
   if (c->batch > 0 && (!c->kv_lens || (c->max_pages > 0 && !c->page_table)))
     return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: null page table or lengths", who);
+  if ((reinterpret_cast<uintptr_t>(c->kv_lens) | reinterpret_cast<uintptr_t>(c->page_table)) & 3)
+    return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: misaligned page table or lengths", who);
   if (c->batch > 1 && c->table_stride < c->max_pages)
     return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: the page table's rows overlap", who);
   if (c->batch > 0 && c->num_pages < 1) return set_error(LSC_ERROR_INVALID_ARGUMENT, "%s: a cache without pages", who);
@@ -81,7 +83,7 @@ __global__ void __launch_bounds__(256)
     int lo = 0, hi = c.batch;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (__ldg(offsets + mid) <= t) lo = mid;
+      if (offsets[mid] <= t) lo = mid;
       else hi = mid;
     }
     int32_t begin, end;
@@ -93,7 +95,7 @@ __global__ void __launch_bounds__(256)
       if (r == 0) raise_bad_arg(c.err);
       continue;
     }
-    const int32_t page = __ldg(c.table + lo * c.table_stride + (pos >> c.page_shift));
+    const int32_t page = c.table[lo * c.table_stride + (pos >> c.page_shift)];
     if (page < 0 || page >= c.num_pages) {
       if (r == 0) raise_bad_arg(c.err);
       continue;
@@ -101,8 +103,8 @@ __global__ void __launch_bounds__(256)
     const int64_t src = t * new_token + h * new_head + e;
     const int64_t dst = page * c.page_stride + (pos & ((1 << c.page_shift) - 1)) * c.token_stride +
                         h * c.head_stride + e;
-    const uint4 kv = __ldg(reinterpret_cast<const uint4*>(k_new + src));
-    const uint4 vv = __ldg(reinterpret_cast<const uint4*>(v_new + src));
+    const uint4 kv = *reinterpret_cast<const uint4*>(k_new + src);
+    const uint4 vv = *reinterpret_cast<const uint4*>(v_new + src);
     *reinterpret_cast<uint4*>(c.k + dst) = kv;
     *reinterpret_cast<uint4*>(c.v + dst) = vv;
   }
@@ -118,10 +120,12 @@ extern "C" lsc_status lsc_kv_cache_append(const lsc_paged_kv* cache, const void*
   PagedView c;
   lsc_status st = paged_view(cache, "kv_cache_append", &c);
   if (st) return st;
-  if (tokens < 0 || tokens > INT32_MAX)
-    return set_error(LSC_ERROR_INVALID_ARGUMENT, "kv_cache_append: bad token count");
+  if (tokens < 0 || tokens > (1 << 30))
+    return set_error(LSC_ERROR_INVALID_ARGUMENT, "kv_cache_append: bad token count (at most 2^30)");
   if (tokens == 0 || c.batch == 0) return LSC_SUCCESS;
   if (!k_new || !v_new || !q_offsets) return set_error(LSC_ERROR_INVALID_ARGUMENT, "kv_cache_append: null pointer");
+  if (reinterpret_cast<uintptr_t>(q_offsets) & 3)
+    return set_error(LSC_ERROR_INVALID_ARGUMENT, "kv_cache_append: misaligned offsets");
   if ((reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new)) & 15)
     return set_error(LSC_ERROR_INVALID_ARGUMENT, "kv_cache_append: k_new and v_new must be 16-byte aligned");
   if (tokens == 1) new_token_stride = 0;

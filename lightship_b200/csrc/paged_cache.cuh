@@ -27,9 +27,11 @@ lsc_status paged_device(const char* who, DeviceState** ds, PagedView* view);
 
 __device__ __forceinline__ void raise_bad_arg(uint32_t* err) { atomicOr(err, LSC_DEVERR_BAD_ARG); }
 
+// Lengths, tables and offsets are read by plain loads: a kernel whose launch overlaps the one before
+// may share an SM with the writer, which the read-only path does not follow.
 // kv_lens[b], clamped to the table's reach; `flag` raises the error word for a length out of range.
 __device__ __forceinline__ int32_t paged_len(const PagedView& c, int b, bool flag) {
-  const int32_t n = __ldg(c.lens + b);
+  const int32_t n = c.lens[b];
   const int32_t most = c.max_pages << c.page_shift;
   if (n >= 0 && n <= most) return n;
   if (flag) raise_bad_arg(c.err);
@@ -37,17 +39,17 @@ __device__ __forceinline__ int32_t paged_len(const PagedView& c, int b, bool fla
 }
 
 // Rows [begin, end) of sequence b among `tokens`; empty where the offsets decrease or leave them.
-__device__ __forceinline__ void query_rows(const int32_t* __restrict__ offsets, int b, int64_t tokens, uint32_t* err,
+__device__ __forceinline__ void query_rows(const int32_t* offsets, int b, int64_t tokens, uint32_t* err,
                                            bool flag, int32_t& begin, int32_t& end) {
-  begin = __ldg(offsets + b);
-  end = __ldg(offsets + b + 1);
+  begin = offsets[b];
+  end = offsets[b + 1];
   if (begin >= 0 && begin <= end && end <= tokens) return;
   if (flag) raise_bad_arg(err);
   end = begin = 0;
 }
 
 // Raises the error word for offsets and lengths out of range; called by the threads of one CTA.
-__device__ __forceinline__ void check_rows(const PagedView& c, const int32_t* __restrict__ offsets, int64_t tokens) {
+__device__ __forceinline__ void check_rows(const PagedView& c, const int32_t* offsets, int64_t tokens) {
   int32_t begin, end;
   for (int b = threadIdx.x; b < c.batch; b += blockDim.x) {
     query_rows(offsets, b, tokens, c.err, true, begin, end);

@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kWalkThreads) rmsnorm_walk_kernel(const RmsArg
     for (int64_t i = threadIdx.x; i < a.d; i += kWalkThreads) {
       const float h = res ? __fadd_rn(ld1(x + i), ld1(res + i)) : ld1(x + i);
       ss = fmaf(h, h, ss);
-      top = fmaxf(top, fabsf(a.gamma ? h * __ldg(a.gamma + i) : h));
+      top = fmaxf(top, fabsf(a.gamma ? h * a.gamma[i] : h));
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kWalkThreads) rmsnorm_walk_kernel(const RmsArg
 #pragma unroll 4
     for (int64_t i = threadIdx.x; i < a.d; i += kWalkThreads) {
       const float h = res ? __fadd_rn(ld1(x + i), ld1(res + i)) : ld1(x + i);
-      const float y = a.gamma ? h * inv * __ldg(a.gamma + i) : h * inv;
+      const float y = a.gamma ? h * inv * a.gamma[i] : h * inv;
       if (a.sum_out) st1(static_cast<TR*>(a.sum_out) + r * a.sum_stride + i, h);
       if (a.out) st1(static_cast<TX*>(a.out) + r * a.out_stride + i, y);
       if (a.q)

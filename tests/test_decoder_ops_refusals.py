@@ -41,7 +41,8 @@ def _decode(cache, q=PTR, heads=4, ts=256, hs=64, alpha=0.125, window=0, sinks=0
     (dict(batch=65536), _lib.ERROR_INVALID_ARGUMENT), (dict(max_pages=-1), _lib.ERROR_INVALID_ARGUMENT),
     (dict(max_pages=1 << 27, table_stride=1 << 27), _lib.ERROR_INVALID_ARGUMENT),
     (dict(kv_lens=None), _lib.ERROR_INVALID_ARGUMENT), (dict(page_table=None), _lib.ERROR_INVALID_ARGUMENT),
-    (dict(table_stride=3), _lib.ERROR_INVALID_ARGUMENT), (dict(k=None), _lib.ERROR_INVALID_ARGUMENT),
+    (dict(kv_lens=PTR + 2), _lib.ERROR_INVALID_ARGUMENT), (dict(page_table=PTR + 1), _lib.ERROR_INVALID_ARGUMENT),
+    (dict(num_pages=0), _lib.ERROR_INVALID_ARGUMENT), (dict(table_stride=3), _lib.ERROR_INVALID_ARGUMENT), (dict(k=None), _lib.ERROR_INVALID_ARGUMENT),
     (dict(v=PTR + 8), _lib.ERROR_INVALID_ARGUMENT), (dict(token_stride=132), _lib.ERROR_INVALID_ARGUMENT),
     (dict(head_stride=32), _lib.ERROR_INVALID_ARGUMENT), (dict(page_stride=-8), _lib.ERROR_INVALID_ARGUMENT),
 ])
@@ -66,7 +67,8 @@ def test_no_cache_refused():
 
 
 @pytest.mark.parametrize("kw", [dict(tokens=-1), dict(k=None), dict(v=None), dict(off=None), dict(k=PTR + 2),
-                                dict(ts=130), dict(hs=4), dict(ts=-128)])
+                                dict(ts=130), dict(hs=4), dict(ts=-128),
+                                dict(off=PTR + 2), dict(tokens=(1 << 30) + 1)])
 def test_append_refusals(kw):
     assert _append(_cache(), **kw) == _lib.ERROR_INVALID_ARGUMENT
 
@@ -77,7 +79,8 @@ BOTH = [dict(heads=3), dict(heads=0), dict(alpha=0.0), dict(alpha=-1.0), dict(al
         dict(i8=PTR, s=float("nan"))]
 
 
-@pytest.mark.parametrize("kw", BOTH + [dict(off=None), dict(tokens=-1)])
+@pytest.mark.parametrize("kw", BOTH + [dict(off=None), dict(off=PTR + 1), dict(tokens=-1),
+                                       dict(tokens=(1 << 30) + 1)])
 def test_prefill_refusals(kw):
     assert _prefill(_cache(), **kw) == _lib.ERROR_INVALID_ARGUMENT
 

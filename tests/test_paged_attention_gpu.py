@@ -490,3 +490,105 @@ def test_prompt_chunks_and_tokens_agree(cuda):
     step = 4 * s_o * float(np.abs(wo).max())
     for chunks in ([20, 2, 33, 20], [70] + [1] * 5, [1] * 10 + [65]):
         assert float((run(chunks) - whole).abs().max()) <= step
+
+
+def test_captured_token_steps(cuda):
+    """One captured step - the lengths move on, the new keys and values are appended, the new token attends -
+    replayed over many tokens, across page and tile borders, on top of other launches that overlap."""
+    import torch
+    from lightship_b200 import ops
+    from lightship_b200.kv_cache import PagedKVCache
+    heads, group, d, page, batch, steps = 2, 4, 128, 16, 3, 150
+    g = torch.Generator().manual_seed(6)
+    start = [0, 50, 700]
+    most = -(-(max(start) + steps) // page)
+    k = torch.full((batch * most + 1, page, heads, d), float("nan"), dtype=torch.float16, device=cuda)
+    v = torch.full_like(k, float("nan"))
+    table = torch.randperm(batch * most, generator=g)[:batch * most].view(batch, most).int().to(cuda)
+    lens = torch.zeros(batch, dtype=torch.int32, device=cuda)
+    cache = PagedKVCache(k, v, table, lens)
+    keys = [torch.randn(n + steps, heads, d, generator=g).half().to(cuda) for n in start]
+    values = [torch.randn(n + steps, heads, d, generator=g).half().to(cuda) for n in start]
+    lens.copy_(torch.tensor(start, dtype=torch.int32))
+    off = torch.tensor([0] + start, dtype=torch.int32).cumsum(0).int().to(cuda)
+    cache.append(torch.cat([x[:n] for x, n in zip(keys, start)]), torch.cat([x[:n] for x, n in zip(values, start)]), off)
+    one = torch.arange(batch + 1, dtype=torch.int32, device=cuda)
+    kn = torch.empty(batch, heads, d, dtype=torch.float16, device=cuda)
+    vn, q, x = torch.empty_like(kn), torch.empty(batch, heads * group, d, dtype=torch.float16, device=cuda), None
+    out = torch.empty_like(q)
+    x = torch.empty(batch, heads * group * d, dtype=torch.float16, device=cuda)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        lens.add_(1)
+        cache.append(kn, vn, one)
+        ops.rmsnorm(q.view(batch, -1), out=x)
+        cache.decode(q, out=out)
+    for t in range(steps):
+        kn.copy_(torch.stack([y[n + t] for y, n in zip(keys, start)]))
+        vn.copy_(torch.stack([y[n + t] for y, n in zip(values, start)]))
+        q.copy_(2 * torch.randn(q.shape, generator=g).half())
+        graph.replay()
+        if t % 7 == 0 or t == steps - 1:
+            now = [(n + t + 1, 1) for n in start]
+            check(out, q, one, [y[:n] for y, (n, _) in zip(keys, now)], [y[:n] for y, (n, _) in zip(values, now)], now,
+                  "float16")
+    assert lens.tolist() == [n + steps for n in start]
+    ops.check_device()
+
+
+def test_two_streams_at_once(cuda):
+    """Prompt and token calls of two caches on two streams, many at a time, give what they give alone."""
+    import torch
+    from lightship_b200 import ops
+    a = make([(3000, 500), (100, 100)], 4, 2, 128, 16, "float16", seed=1)
+    b = make([(5000, 1), (800, 1), (1, 1)], 4, 4, 64, 32, "bfloat16", seed=2)
+    want = a[0].prefill(a[1], a[2]), b[0].decode(b[1])
+    torch.cuda.synchronize()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    got = [[], []]
+    for _ in range(20):
+        with torch.cuda.stream(streams[0]):
+            got[0].append(a[0].prefill(a[1], a[2]))
+        with torch.cuda.stream(streams[1]):
+            got[1].append(b[0].decode(b[1]))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
+    ops.check_device()
+
+
+def test_first_call_inside_a_capture(cuda):
+    """A process whose first use of the operators is a graph capture."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path.insert(0, %r)
+from lightship_b200 import ops
+from lightship_b200.kv_cache import PagedKVCache
+k = torch.randn(40, 16, 2, 64, device="cuda").half()
+v = torch.randn_like(k)
+lens = torch.tensor([600], dtype=torch.int32, device="cuda")
+cache = PagedKVCache(k, v, torch.arange(40, dtype=torch.int32, device="cuda")[None], lens)
+q = torch.randn(1, 4, 64, device="cuda").half()
+off = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+new = torch.randn(1, 2, 64, device="cuda").half()
+outs = [torch.zeros_like(q) for _ in range(2)]
+x = torch.randn(3, 64, device="cuda")
+y = torch.empty_like(x)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    ops.rmsnorm(x, out=y)
+    cache.append(new, new, off)
+    cache.prefill(q, off, out=outs[0])
+    cache.decode(q, out=outs[1])
+g.replay()
+torch.cuda.synchronize()
+assert float((outs[0] - outs[1]).abs().max()) < 4e-3 and float(outs[0].abs().max()) > 0
+assert torch.allclose(y, x / (x.square().mean(1, keepdim=True) + 1e-5).sqrt(), atol=1e-5)
+ops.check_device()
+""" % os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
