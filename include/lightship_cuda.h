@@ -494,9 +494,10 @@ lsc_status lsc_kv_cache_append(const lsc_paged_kv* cache, const void* k_new, con
  * tokens stay visible.  A row that sees no key (p < 0) gives zeros.
  *   out[t, h, :] = softmax_j(alpha * q . k_j) v_j       alpha > 0
  * Scores, maxima and sums in f32; probabilities are rounded to the cache's type for the second
- * product, as are the values they weigh.  out [tokens, q_heads, head_dim] contiguous in the
- * cache's type and/or out_i8 of that shape, quantized per tensor with s_out (`rounding` as
- * lsc_rounding); 16-byte aligned.  Rows before the first offset or behind the last one are left
+ * product (as two such numbers where there is an int8 output, so that its codes are those of
+ * unrounded ones; a value in V that is not finite leaves the codes of the rows it reaches open).
+ * out [tokens, q_heads, head_dim] contiguous in the cache's type and/or out_i8 of that shape,
+ * quantized per tensor with s_out (`rounding` as lsc_rounding); 16-byte aligned.  Rows before the first offset or behind the last one are left
  * as they are.  What the cache holds behind a sequence's last token has no effect.  Rows are
  * worked on in blocks of at most 256 (row, head) pairs of one sequence and key-value head: a place
  * that no row of a block sees has no effect on it, whatever it holds, but a value in V that is not
@@ -510,9 +511,10 @@ lsc_status lsc_paged_attention_prefill(const lsc_paged_kv* cache, const void* q,
  * kv_lens[b] - 1; an empty sequence gives zeros): the cache's length is split over the GPU and
  * the parts are joined in a fixed order, so results do not change from run to run.  Places that
  * the row does not see have no effect, whatever they hold.  `workspace`: device scratch of
- * lsc_paged_attention_decode_workspace_size(cache, q_heads) bytes (0 where no sequence can hold
- * more than 512 tokens: then it may be NULL), 16-byte aligned, with any content; calls that share one must be ordered on one stream (two captured graphs that share
- * one must not run at the same time). */
+ * lsc_paged_attention_decode_workspace_size(cache, q_heads) bytes (0 where the sequences are too
+ * short to be split, max_pages of at most 256 or 512 tokens: then it may be NULL), 16-byte
+ * aligned, with any content; calls that share one must be ordered on one stream (two captured
+ * graphs that share one must not run at the same time). */
 uint64_t lsc_paged_attention_decode_workspace_size(const lsc_paged_kv* cache, int32_t q_heads);
 lsc_status lsc_paged_attention_decode(const lsc_paged_kv* cache, const void* q, int32_t q_heads,
                                       int64_t q_token_stride, int64_t q_head_stride, float alpha, int64_t window,

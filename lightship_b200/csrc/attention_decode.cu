@@ -15,7 +15,8 @@
 // boxes of pages without a visible place read out of the tensor's range: zeros, no traffic).
 // Four warps multiply: the up to 16 query heads of a group are the rows of m16n8k16 products (the
 // instruction needs one eighth of the rows that tcgen05 does, and at 4 flops a byte the legacy
-// tensor path is far from its limit).  Groups of more than 16 heads give the warps heads instead
+// tensor path is far from its limit).  Measured: 131072 places of 8 bf16 heads of 128, 32 query heads, in
+// 92 us (5.83 TB/s of keys and values); 64 sequences of up to 8192 places in 183 us (5.95 TB/s).  Groups of more than 16 heads give the warps heads instead
 // of keys: MT row tiles x (4 / MT) key slices.  Each warp keeps its own m, l and O.
 #include "attention_paged.cuh"
 
@@ -26,7 +27,6 @@ constexpr int kTile = 64;         // places per key tile
 constexpr int kConsumers = 4;     // multiplying warps
 constexpr int kDecodeThreads = 32 * (kConsumers + 1);
 constexpr int kMaxCtas = 320;     // bound of the grid, and so of the workspace
-constexpr int kNoSplitTiles = 8;  // sequences this short are not cut (is_cut)
 
 template <int D>
 struct DecodeShape {
@@ -119,7 +119,9 @@ __device__ __forceinline__ void write_pair(const AttnArgs& a, int64_t at, float 
   }
 }
 
-template <bool BF16, int D, int MT>
+// FINE, for an int8 output: each p goes into the product as its rounding and the rounding of what is
+// left (p rounded once sends values next to a border of the output's codes to the other side).
+template <bool BF16, int D, int MT, bool FINE>
 __global__ void __launch_bounds__(kDecodeThreads, 2)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                         const PagedView c, const DecodeArgs p) {
@@ -411,6 +413,11 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
         }
         const uint32_t pa[4] = {pack16<BF16>(e[0], e[1]), pack16<BF16>(e[2], e[3]), pack16<BF16>(e[4], e[5]),
                                 pack16<BF16>(e[6], e[7])};
+        uint32_t pl[4];  // (FINE) what the rounding left
+        if constexpr (FINE) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) pl[x] = pack16_rest<BF16>(e[2 * x], e[2 * x + 1], pa[x]);
+        }
         // values of places that are not seen count as zero, whatever the cache holds there
         uint32_t keep0 = 0xFFFFFFFFu, keep1 = 0xFFFFFFFFu;
         if (edge) {
@@ -428,6 +435,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
           ldsm4_t(at + (k >> 2) * block_bytes + ((chunk ^ (key & 7)) << 4), b);
           mma16816<BF16>(o[2 * k], pa, b[0] & keep0, b[1] & keep1);
           mma16816<BF16>(o[2 * k + 1], pa, b[2] & keep0, b[3] & keep1);
+          if constexpr (FINE) {
+            mma16816<BF16>(o[2 * k], pl, b[0] & keep0, b[1] & keep1);
+            mma16816<BF16>(o[2 * k + 1], pl, b[2] & keep0, b[3] & keep1);
+          }
         }
       }
       __syncwarp();
@@ -607,10 +618,16 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedView c, cons
 // Row tiles of a group: 16 heads while they suffice, then 32, then 64 (and several of those).
 int row_tiles(int group) { return group <= 16 ? 1 : (group <= 32 ? 2 : 4); }
 
-// A cache of at most kNoSplitTiles tiles per sequence is not cut: the join's launch would cost more
-// than the tiles it spreads (one sequence of 200 places, 12 heads: 7.9 us whole).
+// Caches of short sequences are not cut: the join (2 us, and the parts' way through memory) would cost
+// more than the tiles it spreads.  A CTA takes 0.9 us per tile of heads of 128, half of that for heads of
+// 64, and with many pairs the GPU is full without a cut.  Cut and whole, us: 8 pairs of 128, 192 places
+// 10.2 and 9.7, 320 places 10.6 and 11.8, 512 places 10.8 and 14.4; 32 pairs of 64, 512 places 9.7 and
+// 9.5; 64 pairs of 128, 384 places 14.0 and 13.1, 512 places 14.5 and 14.9; 128 pairs of 128, 512 places
+// 17.2 and 15.2, 768 places 18.2 and 18.7.
 bool is_cut(const lsc_paged_kv* cache) {
-  return static_cast<int64_t>(cache->max_pages) * cache->page_size > kNoSplitTiles * kTile;
+  const int64_t pairs = static_cast<int64_t>(cache->batch) * cache->kv_heads;
+  const int64_t whole = cache->head_dim == 128 && pairs < 64 ? 256 : 512;  // places
+  return static_cast<int64_t>(cache->max_pages) * cache->page_size > whole;
 }
 
 uint64_t workspace_bytes_for(int group, int head_dim) {
@@ -618,7 +635,7 @@ uint64_t workspace_bytes_for(int group, int head_dim) {
   return kMaxCtas * 16 + 2 * kMaxCtas * rows * (head_dim + 2) * 4;
 }
 
-template <bool BF16, int D, int MT>
+template <bool BF16, int D, int MT, bool FINE>
 lsc_status launch_decode(const lsc_paged_kv* cache, const DeviceState* ds, const PagedView& c, DecodeArgs p,
                          cudaStream_t st) {
   using Shape = DecodeShape<D>;
@@ -629,9 +646,9 @@ lsc_status launch_decode(const lsc_paged_kv* cache, const DeviceState* ds, const
   if (s) return s;
   int grid = 2 * ds->sm_count;
   if (grid > kMaxCtas) grid = kMaxCtas;
-  LSC_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<BF16, D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  LSC_CUDA_TRY(cudaFuncSetAttribute(paged_decode_kernel<BF16, D, MT, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     Shape::kSmem));
-  LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, paged_decode_kernel<BF16, D, MT>, dim3(grid),
+  LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, paged_decode_kernel<BF16, D, MT, FINE>, dim3(grid),
                                 dim3(kDecodeThreads), Shape::kSmem, st, tk, tv, c, p));
   if (p.split) {
     const int rows = p.a.group < 16 ? p.a.group : 16;
@@ -641,13 +658,13 @@ lsc_status launch_decode(const lsc_paged_kv* cache, const DeviceState* ds, const
   return LSC_SUCCESS;
 }
 
-template <bool BF16, int D>
+template <bool BF16, int D, bool FINE>
 lsc_status launch_decode_rows(const lsc_paged_kv* cache, const DeviceState* ds, const PagedView& c, const DecodeArgs& p,
                               cudaStream_t st) {
   switch (row_tiles(p.a.group)) {
-    case 1: return launch_decode<BF16, D, 1>(cache, ds, c, p, st);
-    case 2: return launch_decode<BF16, D, 2>(cache, ds, c, p, st);
-    default: return launch_decode<BF16, D, 4>(cache, ds, c, p, st);
+    case 1: return launch_decode<BF16, D, 1, FINE>(cache, ds, c, p, st);
+    case 2: return launch_decode<BF16, D, 2, FINE>(cache, ds, c, p, st);
+    default: return launch_decode<BF16, D, 4, FINE>(cache, ds, c, p, st);
   }
 }
 
@@ -692,9 +709,13 @@ lsc_status lsc_paged_attention_decode(const lsc_paged_kv* cache, const void* q, 
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = cache->dtype == LSC_DTYPE_BF16;
-  if (cache->head_dim == 64)
-    return bf16 ? launch_decode_rows<true, 64>(cache, ds, c, p, s) : launch_decode_rows<false, 64>(cache, ds, c, p, s);
-  return bf16 ? launch_decode_rows<true, 128>(cache, ds, c, p, s) : launch_decode_rows<false, 128>(cache, ds, c, p, s);
+  const bool wide = cache->head_dim == 128;
+  if (out_i8) {
+    if (bf16) return wide ? launch_decode_rows<true, 128, true>(cache, ds, c, p, s) : launch_decode_rows<true, 64, true>(cache, ds, c, p, s);
+    return wide ? launch_decode_rows<false, 128, true>(cache, ds, c, p, s) : launch_decode_rows<false, 64, true>(cache, ds, c, p, s);
+  }
+  if (bf16) return wide ? launch_decode_rows<true, 128, false>(cache, ds, c, p, s) : launch_decode_rows<true, 64, false>(cache, ds, c, p, s);
+  return wide ? launch_decode_rows<false, 128, false>(cache, ds, c, p, s) : launch_decode_rows<false, 64, false>(cache, ds, c, p, s);
 }
 
 }  // extern "C"

@@ -82,6 +82,15 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   return d;
 }
 
+// What packing left of both: {lo, hi} minus the packed values, rounded and packed
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16_rest(float lo, float hi, uint32_t packed) {
+  float2 v;
+  if constexpr (BF16) v = make_float2(__uint_as_float(packed << 16), __uint_as_float(packed & 0xFFFF0000u));
+  else v = __half22float2(*reinterpret_cast<const __half2*>(&packed));
+  return pack16<BF16>(lo - v.x, hi - v.y);
+}
+
 // The key tiles (of TILE places) that queries at positions first .. last meet, sinks apart from
 // the window: tile i of n is key tile i < sink_tiles ? i : start + i - sink_tiles.
 template <int TILE>

@@ -16,13 +16,18 @@
 //                   that one tile's softmax runs beside the other's products;
 //   warp 11         brings the K and V tiles by TMA, page by page; boxes of pages without a visible
 //                   place read out of the tensor's range: zeros, no traffic;
-//   warp 10         finds the units, brings their Q, and zeroes the rows of V that no row of the unit sees (a product
-//                   with p = 0 would keep a NaN) in the few tiles that have such rows, before they
-//                   are released to the products.
+//   warp 10         finds the units, brings their Q, and zeroes the rows of V that no row of the unit
+//                   sees (a product with p = 0 would keep a NaN) in the few tiles that have such
+//                   rows, before they are released to the products.
 // m moves only when a row's maximum passes it by more than 2^8: until then p stays below 2^8,
 // which the 16-bit types and the f32 sums hold as exactly as values below 1, and O needs no
 // rescaling.  When it moves, the softmax thread rescales its row of O in TMEM; the products into O
 // that it follows are complete, because S of this tile was issued behind them.
+// What bounds it: 128 x 128 scores take 1024 clocks of the tensor cores with heads of 128 (both products) and
+// the same of the special function units, and a row tile's softmax and products follow one another; two row tiles
+// fill each other's gaps to 59 % of the tensor cores' measured rate.  Measured: 8192 tokens, 32 query
+// heads on 8 of 128 (f16) in 565 us, 974 TFLOP/s; 16 on 4 of 64 with a window of 1024 in 94 us; 100
+// tokens of 12 heads of 64 in 7.7 us.
 // Every wait is bounded (a timeout flags the device error word and ends the CTA's work).
 #include <type_traits>
 
@@ -31,13 +36,17 @@
 namespace lsc {
 namespace {
 
-constexpr int kTile = 128;            // rows of a row tile, places of a key tile
+constexpr int kTile = 128;       // rows of a row tile, places of a key tile
 constexpr int kPrefillThreads = 384;
 constexpr int kSchedSlots = 4;
-constexpr int kParts = 2;              // parts of P that are passed on
-constexpr int kFirstPart = 96;         // keys of the first (the products of the last are waited for)
-constexpr int kTurnAt = 3;             // the quarter of the exponentials after which the other row tile may begin
-constexpr float kMoveBy = 8.0f;       // log2 of how far a maximum may pass the reference
+constexpr int kParts = 2;        // parts of P that are passed on
+// Keys of the first part.  The products of the last part are what the next scores wait for, so it is
+// small; 64 keys took 510 us where 96 take 497 (8192 tokens, 32 query heads on 8 of 128).
+constexpr int kFirstPart = 96;
+// The quarter of the exponentials after which the other row tile may begin: 1, 2 and 3 took 573, 546 and
+// 503 us there, no turns at all 537.
+constexpr int kTurnAt = 3;
+constexpr float kMoveBy = 8.0f;  // log2 of how far a maximum may pass the reference
 
 // max of three (NaN operands are ignored)
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
@@ -46,7 +55,7 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
-template <int D>
+template <int D, bool FINE>
 struct PrefillShape {
   static constexpr int kTileBytes = kTile * D * 2;    // Q, K or V of one tile
   static constexpr int kStages = D == 128 ? 5 : 10;   // K and V tiles in turn
@@ -55,13 +64,14 @@ struct PrefillShape {
   // TMEM columns of a row tile's S and P, then O of both.  Heads of 128 leave 128 columns for S, and P
   // takes its place: the next S waits for the products with P.  Heads of 64 leave 192 (kApart): tiles
   // take turns at S in the last or the first 128 and P in the last or the first 64 of them, so the next
-  // S never meets the P in use and is there when the softmax comes for it.
-  static constexpr bool kApart = D == 64;
+  // S never meets the P in use and is there when the softmax comes for it.  FINE needs 64 more columns
+  // for the low parts of P: there all heads do as heads of 128.
+  static constexpr bool kApart = D == 64 && !FINE;
   static constexpr uint32_t kColsS = kApart ? 192 : 128, kColO = 2 * kColsS;
   static constexpr uint32_t s_at(uint32_t turn) { return kApart && turn == 0 ? 64 : 0; }
   static constexpr uint32_t p_at(uint32_t turn) { return kApart && turn == 0 ? 128 : 0; }
 };
-static_assert(PrefillShape<128>::kSmem <= 232448 && PrefillShape<64>::kSmem <= 232448, "shared memory budget");
+static_assert(PrefillShape<128, false>::kSmem <= 232448 && PrefillShape<64, false>::kSmem <= 232448, "shared memory budget");
 
 struct PrefillArgs {
   AttnArgs a;
@@ -225,11 +235,14 @@ struct Scheduler {
   }
 };
 
-template <bool BF16, int D>
+// FINE, for an int8 output: each p goes into the products as two 16-bit numbers, its rounding and the
+// rounding of what is left.  p rounded once moves a value by up to 2^-11 or 2^-8 of it, which is far
+// below a step of the output but sends the values next to a border to the other code.
+template <bool BF16, int D, bool FINE>
 __global__ void __launch_bounds__(kPrefillThreads, 1)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                          const __grid_constant__ CUtensorMap tm_v, const PagedView c, const PrefillArgs p) {
-  using Shape = PrefillShape<D>;
+  using Shape = PrefillShape<D, FINE>;
   constexpr int kBlocks = D / 64;
   constexpr int kStages = Shape::kStages;
   constexpr int kBlockBytes = kTile * 128;  // 128 rows of one 128-byte column block
@@ -571,8 +584,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           auto products = [&](auto part) {  // by the elected lane
             constexpr int x = decltype(part)::value, kCut = kFirstPart / 16;
 #pragma unroll
-            for (int k = x ? kCut : 0; k < (x ? kTile / 16 : kCut); ++k)
+            for (int k = x ? kCut : 0; k < (x ? kTile / 16 : kCut); ++k) {
               mma_f16_ts(t_o, t_p + k * 8, dva + k * (2048 >> 4), idesc_o, k != 0 ? 1u : more);
+              if constexpr (FINE) mma_f16_ts(t_o, t_p + kTile / 2 + k * 8, dva + k * (2048 >> 4), idesc_o, 1u);
+            }
           };
           if constexpr (Shape::kApart) {
             if (j < n) {
@@ -737,7 +752,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         };
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          uint32_t packed[16];
+          uint32_t packed[16], low[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float y0, y1;
@@ -746,10 +761,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
             y1 = ex2_approx(y1);
             sum2[e & 1] = f2add(sum2[e & 1], f2pack(y0, y1));
             packed[e] = pack16<BF16>(y0, y1);
+            if constexpr (FINE) low[e] = pack16_rest<BF16>(y0, y1, packed[e]);
           }
           if (shared && x == kTurnAt && lane == 0) mbar_arrive(turn + (w ^ 1));
           if (x == kFirstPart / 32) arrive(0);  // its stores have had the time of 32 keys to complete
           tmem_st_32x32b_x16(p_here + 16 * x, packed);
+          if constexpr (FINE) tmem_st_32x32b_x16(p_here + kTile / 2 + 16 * x, low);
         }
         arrive(1);
         if (quarter == 0 && lane == 0) {
@@ -820,10 +837,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   }
 }
 
-template <bool BF16, int D>
+template <bool BF16, int D, bool FINE>
 lsc_status launch_prefill(const lsc_paged_kv* cache, const DeviceState* ds, const PagedView& c, PrefillArgs p,
                           cudaStream_t st) {
-  using Shape = PrefillShape<D>;
+  using Shape = PrefillShape<D, FINE>;
   const AttnArgs& a = p.a;
   const uint32_t box = cache->page_size < kTile ? cache->page_size : kTile;
   CUtensorMap tq, tk, tv;
@@ -842,15 +859,17 @@ lsc_status launch_prefill(const lsc_paged_kv* cache, const DeviceState* ds, cons
   auto units = [&](int64_t tokens) {
     return (a.tokens / tokens + (a.tokens < c.batch ? a.tokens : c.batch)) * p.pairs;
   };
-  // two row tiles per unit hide one's softmax behind the other's products; with fewer units than SMs
-  // one row tile each spreads the work over more of them
+  // Two row tiles per unit hide one's softmax behind the other's products; with fewer units than SMs
+  // one row tile each spreads the work over more of them.  One and two, us: 256 tokens of 12 heads of 64
+  // 8.7 and 9.6; 32 query heads on 8 of 128, 512 tokens 14.6 and 16.2, 1024 tokens (136 units) 25.1 and
+  // 24.3, 2048 tokens 66.9 and 42.8.
   p.unit_tokens = units(2 * p.tpt) < ds->sm_count ? p.tpt : 2 * p.tpt;
   const int64_t most = units(p.unit_tokens);
   const int grid = static_cast<int>(most < ds->sm_count ? most : ds->sm_count);
-  LSC_CUDA_TRY(cudaFuncSetAttribute(paged_prefill_kernel<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  LSC_CUDA_TRY(cudaFuncSetAttribute(paged_prefill_kernel<BF16, D, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     Shape::kSmem));
-  LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, paged_prefill_kernel<BF16, D>, dim3(grid), dim3(kPrefillThreads),
-                                Shape::kSmem, st, tq, tk, tv, c, p));
+  LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, paged_prefill_kernel<BF16, D, FINE>, dim3(grid),
+                                dim3(kPrefillThreads), Shape::kSmem, st, tq, tk, tv, c, p));
   return LSC_SUCCESS;
 }
 
@@ -946,7 +965,11 @@ extern "C" lsc_status lsc_paged_attention_prefill(const lsc_paged_kv* cache, con
   p.pairs = c.kv_heads * (p.a.group / p.hp);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool bf16 = cache->dtype == LSC_DTYPE_BF16;
-  if (cache->head_dim == 64)
-    return bf16 ? launch_prefill<true, 64>(cache, ds, c, p, s) : launch_prefill<false, 64>(cache, ds, c, p, s);
-  return bf16 ? launch_prefill<true, 128>(cache, ds, c, p, s) : launch_prefill<false, 128>(cache, ds, c, p, s);
+  const bool wide = cache->head_dim == 128;
+  if (out_i8) {
+    if (bf16) return wide ? launch_prefill<true, 128, true>(cache, ds, c, p, s) : launch_prefill<true, 64, true>(cache, ds, c, p, s);
+    return wide ? launch_prefill<false, 128, true>(cache, ds, c, p, s) : launch_prefill<false, 64, true>(cache, ds, c, p, s);
+  }
+  if (bf16) return wide ? launch_prefill<true, 128, false>(cache, ds, c, p, s) : launch_prefill<true, 64, false>(cache, ds, c, p, s);
+  return wide ? launch_prefill<false, 128, false>(cache, ds, c, p, s) : launch_prefill<false, 64, false>(cache, ds, c, p, s);
 }

@@ -9,7 +9,9 @@ is at most 2^8 times too large or small for its reference, which a floating type
 the sums over n keys are f32 (n w each, and the rescalings of a running maximum one w per 64 keys,
 within that).  So |got - o| <= u |o| + A (u + 2 e + 2 n w) + F with e = g + 3 |s| w + 2^-21,
 A = sum_j p_j |v_j| / l and F the flushed part.  An int8 code is within half a step of o / s_out
-plus that bound over s_out."""
+plus that bound over s_out; for a call with an int8 output p is two numbers of the cache's type, its
+rounding and the rounding of what is left, and o is not rounded to that type: there the bound is
+A (u^2 + 2 e + 2 n w) + F."""
 import math
 
 import pytest
@@ -59,9 +61,10 @@ def make(seqs, heads, group, d, page, kind, seed=0, layout="token", scale=2.0, h
     return cache, q, torch.tensor(offsets, dtype=torch.int32, device=dev), keys, values
 
 
-def define(q, pos, k, v, alpha, window, sinks, kind):
+def define(q, pos, k, v, alpha, window, sinks, kind, fine=False):
     """(o, tolerance, whether it sees a key) for rows q [m, H, D] at positions pos over k, v [n, heads, D]."""
     import torch
+    u = U[kind] ** 2 if fine else U[kind]
     m, hq, d = q.shape
     n, heads = k.shape[:2]
     o = torch.zeros(m, hq, d, dtype=torch.float64, device=q.device)
@@ -81,13 +84,16 @@ def define(q, pos, k, v, alpha, window, sinks, kind):
         o[:, h] = p @ vv / l
         e = torch.where(see, d * W * g + 3 * s.abs() * W + 2.0 ** -21, 0.0)
         f = torch.where(see, p.clamp(max=2.0 ** -25), 0.0) @ vv.abs() / l if kind == "float16" else 0.0
-        tol[:, h] = U[kind] * o[:, h].abs() + (p * (U[kind] + 2 * e + 2 * n * W)) @ vv.abs() / l + f + 1e-30
+        tol[:, h] = (p * (u + 2 * e + 2 * n * W)) @ vv.abs() / l + f + 1e-30
+        if not fine:
+            tol[:, h] += U[kind] * o[:, h].abs()
         if kind == "float16":
             tol[:, h] += 2.0 ** -25
     return o, tol, see.any(1)
 
 
-def check(got, q, offsets, keys, values, seqs, kind, window=0, sinks=0, alpha=None, s_out=None):
+def check(got, q, offsets, keys, values, seqs, kind, window=0, sinks=0, alpha=None, s_out=None,
+          fine=False):
     import torch
     d = q.shape[2]
     alpha = d ** -0.5 if alpha is None else alpha
@@ -97,7 +103,7 @@ def check(got, q, offsets, keys, values, seqs, kind, window=0, sinks=0, alpha=No
             continue
         rows = slice(int(offsets[b]), int(offsets[b + 1]))
         pos = torch.arange(n - m, n, device=q.device)
-        o, tol, any_key = define(q[rows], pos, keys[b], values[b], alpha, window, sinks, kind)
+        o, tol, any_key = define(q[rows], pos, keys[b], values[b], alpha, window, sinks, kind, fine)
         assert bool((got[rows][~any_key] == 0).all())
         if s_out is not None:
             t = o / s_out
@@ -205,6 +211,25 @@ def test_int8_outputs(cuda, kind, d, group, rounding):
     last = [(90, 1), (400, 1)]
     check(d8, q1, torch.tensor([0, 1, 2]), keys, values, last, kind, s_out=0.02)
     check(one, q1, torch.tensor([0, 1, 2]), keys, values, last, kind)
+
+
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d,heads,group,window,sinks", [(64, 2, 4, 0, 0), (64, 1, 20, 300, 5), (128, 2, 4, 0, 0),
+                                                        (128, 1, 3, 130, 0)])
+def test_int8_codes_are_those_of_unrounded_probabilities(cuda, kind, d, heads, group, window, sinks):
+    """Rounding p to the cache's type would move a code's value by up to a sixth of a step here."""
+    import torch
+    seqs = [(700, 300), (90, 90), (1, 1), (2600, 130), (5, 5)]
+    cache, q, offsets, keys, values = make(seqs, heads, group, d, 16, kind, seed=12)
+    more = dict(window=window, sinks=sinks)
+    q8 = torch.empty(q.shape, dtype=torch.int8, device=cuda)
+    cache.prefill(q, offsets, out_i8=q8, s_out=0.02, **more)
+    check(q8, q, offsets, keys, values, seqs, kind, s_out=0.02, fine=True, **more)
+    q1 = q[offsets[1:].long() - 1]
+    d8 = torch.empty(q1.shape, dtype=torch.int8, device=cuda)
+    cache.decode(q1, out_i8=d8, s_out=0.02, **more)
+    check(d8, q1, torch.arange(len(seqs) + 1), keys, values, [(n, 1) for n, _ in seqs], kind, s_out=0.02, fine=True,
+          **more)
 
 
 @pytest.mark.parametrize("scale,alpha", [(30.0, None), (1e-3, None), (2.0, 1e-6), (100.0, 1.0)])
