@@ -92,10 +92,11 @@ __device__ __forceinline__ uint32_t pack16_rest(float lo, float hi, uint32_t pac
 }
 
 // The key tiles (of TILE places) that queries at positions first .. last meet, sinks apart from
-// the window: tile i of n is key tile i < sink_tiles ? i : start + i - sink_tiles.
+// the window: tile i of n is key tile i < sink_tiles ? i : start + i - sink_tiles, counted from `skip`
+// on where the list is a part of another.
 template <int TILE>
 struct TileList {
-  int32_t n, sink_tiles, start;
+  int32_t n, sink_tiles, start, skip = 0;
   __device__ __forceinline__ TileList(int32_t first, int32_t last, int32_t window, int32_t sinks) {
     const int32_t low = window > 0 && first >= window ? first - window + 1 : 0;
     const int32_t kept = sinks < low ? sinks : low;
@@ -104,7 +105,15 @@ struct TileList {
     if (start <= sink_tiles) sink_tiles = start = 0;
     n = last < 0 ? 0 : sink_tiles + last / TILE + 1 - start;
   }
-  __device__ __forceinline__ int32_t tile(int32_t i) const { return i < sink_tiles ? i : start + i - sink_tiles; }
+  __device__ __forceinline__ int32_t tile(int32_t i) const {
+    i += skip;
+    return i < sink_tiles ? i : start + i - sink_tiles;
+  }
+  // part x of `parts` equal ones
+  __device__ __forceinline__ void take(int32_t x, int32_t parts) {
+    skip = static_cast<int32_t>(static_cast<int64_t>(n) * x / parts);
+    n = static_cast<int32_t>(static_cast<int64_t>(n) * (x + 1) / parts) - skip;
+  }
 };
 
 }  // namespace lsc

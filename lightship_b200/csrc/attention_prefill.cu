@@ -28,7 +28,12 @@
 // fill each other's gaps to 59 % of the tensor cores' measured rate.  Measured: 8192 tokens, 32 query
 // heads on 8 of 128 (f16) in 565 us, 974 TFLOP/s; 16 on 4 of 64 with a window of 1024 in 94 us; 100
 // tokens of 12 heads of 64 in 7.7 us.
+// With few units (a chunk of a prompt on a long cache) a cluster of 2, 4 or 8 CTAs shares each of them:
+// every CTA takes a part of the unit's key tiles, keeps its own m, l and O, and sends each CTA of the
+// cluster a share of O's columns through distributed shared memory; the shares are joined there in
+// the order of the parts.  No workspace, no second launch.
 // Every wait is bounded (a timeout flags the device error word and ends the CTA's work).
+#include <mutex>
 #include <type_traits>
 
 #include "attention_paged.cuh"
@@ -46,6 +51,7 @@ constexpr int kFirstPart = 96;
 // The quarter of the exponentials after which the other row tile may begin: 1, 2 and 3 took 573, 546 and
 // 503 us there, no turns at all 537.
 constexpr int kTurnAt = 3;
+constexpr int kSharedPlaces = 256;   // places per CTA of a cluster, at least
 constexpr float kMoveBy = 8.0f;  // log2 of how far a maximum may pass the reference
 
 // max of three (NaN operands are ignored)
@@ -79,6 +85,7 @@ struct PrefillArgs {
   int32_t tpt;         // tokens of a tile: 128 / hp
   int32_t unit_tokens; // tokens of a unit: tpt or 2 tpt
   int32_t pairs;       // key-value heads x (group / hp)
+  int32_t parts;       // CTAs of a cluster that share a unit of one row tile; 1: no cluster
 };
 
 // A unit: tokens [row0, row0 + count) of the batch, the first at position pos0 of sequence b.
@@ -113,6 +120,11 @@ struct TileSpan {
     const int32_t sink_tiles = sinks > 0 ? (sinks - 1) / kTile + 1 : 0;
     kept = tiles.sink_tiles > 0 ? tiles.sink_tiles : sink_tiles;
     kept = kept < to ? kept : to;
+    // numbers of the part that the list is
+    auto clip = [&](int32_t i) { return i < tiles.skip ? 0 : (i - tiles.skip < n ? i - tiles.skip : n); };
+    kept = clip(kept);
+    from = clip(from);
+    to = clip(to);
     if (kept >= from) kept = from = 0;
   }
   __device__ __forceinline__ bool has(int32_t i) const { return i < kept || (i >= from && i < to); }
@@ -295,6 +307,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       mbar_init(sched_empty + s, 8 + 2 + 1);  // softmax, products, loads of K and V
     }
     *abort_flag = 0u;
+    sched[0].b = -1;
     fence_barrier_init();
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
@@ -324,7 +337,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     }
     return u.b >= 0;
   };
-  auto tiles_of = [&](const Unit& u) { return TileList<kTile>(u.pos0, u.pos0 + u.count - 1, a.window, a.sinks); };
+  auto tiles_of = [&](const Unit& u) {
+    TileList<kTile> tiles(u.pos0, u.pos0 + u.count - 1, a.window, a.sinks);
+    if (p.parts > 1) tiles.take(static_cast<int32_t>(blockIdx.x % p.parts), p.parts);
+    return tiles;
+  };
 
   if (warp >= 8) {
     regs_shrink<88>();
@@ -369,12 +386,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         if (more && found - zeroed < kSchedSlots &&
             (zeroed == found ||
              __all_sync(0xffffffffu, mbar_test_wait(smem_u32(sched_empty + sched_at), sched_phase ^ 1u)))) {
-          const int64_t i = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+          int64_t i = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+          if (p.parts > 1) i = round == 0 ? blockIdx.x / p.parts : s.total;  // one unit per cluster
           ++round;
           Unit u{};
           u.b = -1;
           if (i < s.total) u = s.find(i);
-          else if ((round - 1) * gridDim.x < s.total) continue;  // the last round has no unit for this CTA
+          else if (p.parts == 1 && (round - 1) * gridDim.x < s.total) continue;  // the last round has none for this CTA
           more = u.b >= 0;
           if (!(ok = warp_wait(sched_empty + sched_at, sched_phase ^ 1u, abort_flag, c.err))) break;
           if (lane == 0) {
@@ -633,6 +651,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         __syncwarp();
       }
     }
+    if (p.parts > 1) {
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
   } else {
     // -------------------------------------------------------------------- softmax and output
     regs_grow<208>();
@@ -646,6 +669,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     uint32_t s_phase = 0, o_phase = 0, last_phase = 0;
     uint32_t stage0 = 0;  // of the unit's first K tile
     uint32_t turn_phase = w == 0 ? 1u : 0u;  // row tile 0 begins
+    float ref = -INFINITY;  // the reference m, in units of the raw scores
+    float l = 0.0f;
+    int done = 0;
     Unit u;
     bool ok = true;
     while (ok && next_unit(u)) {
@@ -664,9 +690,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const int32_t pos = rows.first + (mine ? token : rows.count - 1);
       const int32_t low = a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0;
       const int32_t pos_min = __shfl_sync(0xffffffffu, pos, 0), low_max = __shfl_sync(0xffffffffu, low, 31);
-      float ref = -INFINITY;  // the reference m, in units of the raw scores
-      float l = 0.0f;
-      int done = 0;
+      ref = -INFINITY;
+      l = 0.0f;
+      done = 0;
       int32_t before = -1, before2 = -1;  // the tile before i, and the one before that
       for (int32_t i = span.next(-1); i < tiles.n;) {
         const int32_t j0 = tiles.tile(i) * kTile, after = span.next(i);
@@ -793,6 +819,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         }
         if (done >= 2) last_phase ^= 1u;
       }
+      if (p.parts > 1) break;
       const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
       const int64_t at = (static_cast<int64_t>(u.row0 + w * p.tpt + token) * a.q_heads + u.head0 + head) * D;
 #pragma unroll 1
@@ -828,6 +855,84 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       // the next unit's products into O follow p_full, which this warp signals behind these loads
       tc_fence_before();
     }
+    if (p.parts > 1) {
+      // CTA x of the cluster joins columns [x width, (x + 1) width) of O.  They arrive where the key
+      // tiles were, [part][row][width], 16-byte pieces turned by the row against bank conflicts; m and
+      // l of all parts where Q was.
+      const uint32_t parts = static_cast<uint32_t>(p.parts), width = D / parts, pieces = width / 4;
+      const uint32_t part = blockIdx.x % parts;
+      float2* const s_ml = reinterpret_cast<float2*>(s_q);  // [part][row]
+      __syncwarp();
+      cluster_sync();  // every CTA's products and copies are complete
+      u = sched[0];
+      const bool here = u.b >= 0 && *abort_flag == 0u;
+      if (here && w == 0) {
+        for (uint32_t x = 0; x < parts; ++x)
+          asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
+                           mapa_shared(smem_u32(s_ml + part * kTile + row), x)),
+                       "f"(ref), "f"(l)
+                       : "memory");
+        if (done) {
+#pragma unroll 1
+          for (uint32_t x = 0; x < D / 16; ++x) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(t_o + 16 * x, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+              const uint32_t column = 16 * x + 4 * e, to = column / width, piece = column % width / 4;
+              const uint32_t at = ((part * kTile + row) * pieces + (piece ^ (row & (pieces - 1)))) * 16;
+              asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(mapa_shared(smem_u32(s_kv) + at, to)),
+                           "r"(o[4 * e]), "r"(o[4 * e + 1]), "r"(o[4 * e + 2]), "r"(o[4 * e + 3])
+                           : "memory");
+            }
+          }
+        }
+      }
+      __syncwarp();
+      cluster_sync();
+      if (here) {
+        const uint32_t chunks = width / 8, rows = static_cast<uint32_t>(u.count * p.hp);
+        for (uint32_t i = threadIdx.x; i < rows * chunks; i += 256) {
+          const uint32_t r = i / chunks, piece = (i - r * chunks) * 2;
+          // a part without a visible key has l = 0, and what it holds of O does not count
+          float m = -INFINITY, sum = 0.0f, y[8] = {};
+          for (uint32_t x = 0; x < parts; ++x) {
+            const float2 ml = s_ml[x * kTile + r];
+            if (ml.y != 0.0f) m = fmaxf(m, ml.x);
+          }
+          for (uint32_t x = 0; x < parts; ++x) {
+            const float2 ml = s_ml[x * kTile + r];
+            if (ml.y == 0.0f) continue;
+            const float f = ex2_approx((ml.x - m) * scale);
+            sum += ml.y * f;
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e) {
+              const float4 v = *reinterpret_cast<const float4*>(
+                  s_kv + ((x * kTile + r) * pieces + ((piece + e) ^ (r & (pieces - 1)))) * 16);
+              y[4 * e] += v.x * f;
+              y[4 * e + 1] += v.y * f;
+              y[4 * e + 2] += v.z * f;
+              y[4 * e + 3] += v.w * f;
+            }
+          }
+          const float inv = sum == 0.0f ? 0.0f : __frcp_rn(sum);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] *= inv;
+          const uint32_t t = r / p.hp;
+          const int64_t at = (static_cast<int64_t>(u.row0 + t) * a.q_heads + u.head0 + (r - t * p.hp)) * D + part * width +
+                             4 * piece;
+          if (a.out)
+            *reinterpret_cast<uint4*>(a.out + at) = make_uint4(pack16<BF16>(y[0], y[1]), pack16<BF16>(y[2], y[3]),
+                                                               pack16<BF16>(y[4], y[5]), pack16<BF16>(y[6], y[7]));
+          if (a.out_i8) {
+            uint32_t pk[2];
+            requant_pack<8>(y, a.s_out, a.inv_s_out, false, a.rounding, pk);
+            *reinterpret_cast<uint2*>(a.out_i8 + at) = make_uint2(pk[0], pk[1]);
+          }
+        }
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -835,6 +940,32 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// Clusters of so many CTAs (2, 4 or 8) that the device runs at the same time
+template <bool BF16, int D, bool FINE>
+lsc_status clusters_at_once(int cluster, int* fit) {
+  static std::once_flag once;
+  static cudaError_t failed = cudaSuccess;
+  static int known[9];
+  std::call_once(once, [] {
+    for (int n = 2; n <= 8 && failed == cudaSuccess; n *= 2) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = static_cast<unsigned>(n);
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.gridDim = dim3(static_cast<unsigned>(n));
+      cfg.blockDim = dim3(kPrefillThreads);
+      cfg.dynamicSmemBytes = PrefillShape<D, FINE>::kSmem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      failed = cudaOccupancyMaxActiveClusters(known + n, paged_prefill_kernel<BF16, D, FINE>, &cfg);
+    }
+  });
+  if (failed != cudaSuccess) return cuda_error(failed, "paged_attention_prefill: clusters");
+  *fit = known[cluster];
+  return LSC_SUCCESS;
 }
 
 template <bool BF16, int D, bool FINE>
@@ -855,21 +986,37 @@ lsc_status launch_prefill(const lsc_paged_kv* cache, const DeviceState* ds, cons
   s = encode_tmap_3d(&tq, BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, a.q, dims, strides,
                      qbox, ones, CU_TENSOR_MAP_SWIZZLE_128B);
   if (s) return s;
-  // units: at most one short one per sequence beside the full ones
+  // units: a sequence's last one may be short
   auto units = [&](int64_t tokens) {
-    return (a.tokens / tokens + (a.tokens < c.batch ? a.tokens : c.batch)) * p.pairs;
+    return (a.tokens + (a.tokens < c.batch ? a.tokens : c.batch) * (tokens - 1)) / tokens * p.pairs;
   };
+  LSC_CUDA_TRY(cudaFuncSetAttribute(paged_prefill_kernel<BF16, D, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                    Shape::kSmem));
   // Two row tiles per unit hide one's softmax behind the other's products; with fewer units than SMs
   // one row tile each spreads the work over more of them.  One and two, us: 256 tokens of 12 heads of 64
   // 8.7 and 9.6; 32 query heads on 8 of 128, 512 tokens 14.6 and 16.2, 1024 tokens (136 units) 25.1 and
   // 24.3, 2048 tokens 66.9 and 42.8.
   p.unit_tokens = units(2 * p.tpt) < ds->sm_count ? p.tpt : 2 * p.tpt;
   const int64_t most = units(p.unit_tokens);
-  const int grid = static_cast<int>(most < ds->sm_count ? most : ds->sm_count);
-  LSC_CUDA_TRY(cudaFuncSetAttribute(paged_prefill_kernel<BF16, D, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    Shape::kSmem));
-  LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, paged_prefill_kernel<BF16, D, FINE>, dim3(grid),
-                                dim3(kPrefillThreads), Shape::kSmem, st, tq, tk, tv, c, p));
+  int grid = static_cast<int>(most < ds->sm_count ? most : ds->sm_count);
+  p.parts = 1;
+  int64_t places = static_cast<int64_t>(c.max_pages) << c.page_shift;
+  const int64_t seen = static_cast<int64_t>(a.window) + a.sinks + p.tpt;
+  if (a.window > 0 && places > seen) places = seen;
+  // A cluster's exchange takes about 6 us, a tile of 128 keys 1.6.  Whole and shared, us, with 8 units:
+  // 512 places 13.0 and (2 parts) 13.5, 1024 places 19.4 and (4) 14.7, 4096 places 57 and (8) 22.5, 65536
+  // places 807 and 121.  More clusters than run at once would take twice the time.
+  if (p.unit_tokens == p.tpt && places >= 1024) {
+    while (p.parts < 8 && 2 * p.parts * kSharedPlaces <= places) {
+      int fit = 0;
+      if ((s = clusters_at_once<BF16, D, FINE>(2 * p.parts, &fit))) return s;
+      if (most > fit) break;
+      p.parts *= 2;
+    }
+  }
+  if (p.parts > 1) grid = static_cast<int>(most) * p.parts;  // units of one row tile: there are few
+  LSC_CUDA_TRY(launch_clusters(ds->overlap_launches, paged_prefill_kernel<BF16, D, FINE>, dim3(grid),
+                               dim3(kPrefillThreads), Shape::kSmem, st, p.parts, tq, tk, tv, c, p));
   return LSC_SUCCESS;
 }
 

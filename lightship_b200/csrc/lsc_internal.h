@@ -34,20 +34,36 @@ struct DeviceState {
 // be scheduled, and run their prologue, while the previous kernel on the stream is finishing.
 // Every kernel launched this way calls griddep_wait() before it reads what an earlier kernel
 // wrote or writes what an earlier kernel may still read.  Graph capture keeps the relation.
+// launch_clusters() launches clusters of `cluster` CTAs (1: no clusters).
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_dependent(bool overlap, void (*kernel)(KArgs...), dim3 grid, dim3 block,
-                                    size_t smem, cudaStream_t stream, Args... args) {
+inline cudaError_t launch_clusters(bool overlap, void (*kernel)(KArgs...), dim3 grid, dim3 block,
+                                   size_t smem, cudaStream_t stream, int cluster, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (overlap) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = overlap ? 1 : 0;
+  cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_dependent(bool overlap, void (*kernel)(KArgs...), dim3 grid, dim3 block,
+                                    size_t smem, cudaStream_t stream, Args... args) {
+  return launch_clusters(overlap, kernel, grid, block, smem, stream, 1, args...);
 }
 
 #ifdef __CUDACC__

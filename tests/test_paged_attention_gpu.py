@@ -163,6 +163,59 @@ def test_prefill_more_units_than_sms(cuda, seqs, heads, group, d, page, window, 
 
 
 @pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1100, 0), (1030, 7), (1500, 2000), (5, 1200)])
+@pytest.mark.parametrize("seqs,heads,group,d,page", [
+    ([(9000, 16)], 8, 4, 128, 64),                                          # 8 units
+    ([(4100, 70), (3, 3), (0, 0), (1500, 1), (2, 5), (129, 129)], 2, 4, 64, 16),
+    ([(2500, 33), (700, 40), (1024, 1)], 1, 3, 128, 256),
+    ([(1025, 200)], 12, 1, 64, 8),
+    ([(3000, 64), (2900, 3), (90, 90)], 5, 8, 128, 32),
+    ([(1300 + 3 * i, 5) for i in range(20)], 1, 2, 64, 16),
+    ([(5000, 3)], 1, 71, 128, 128),
+])
+def test_prefill_few_rows_on_long_caches(cuda, seqs, heads, group, d, page, window, sinks, kind):
+    """A unit's key tiles shared by a cluster: some parts empty, some masked whole, rows without a key."""
+    import torch
+    from lightship_b200 import ops
+    cache, q, offsets, keys, values = make(seqs, heads, group, d, page, kind, seed=heads)
+    more = dict(window=window, sinks=sinks)
+    outs = [torch.full_like(q, 9.0) for _ in range(2)]
+    for out in outs:
+        cache.prefill(q, offsets, out=out, **more)
+    check(outs[0], q, offsets, keys, values, seqs, kind, **more)
+    assert torch.equal(outs[0], outs[1])
+    q8 = torch.empty(q.shape, dtype=torch.int8, device=cuda)
+    cache.prefill(q, offsets, out_i8=q8, s_out=0.02, **more)
+    check(q8, q, offsets, keys, values, seqs, kind, s_out=0.02, fine=True, **more)
+    ops.check_device()
+
+
+def test_prefill_few_rows_back_to_back_and_captured(cuda):
+    """Launches of clusters one behind the other, eager and replayed; rows around the batch stay."""
+    import torch
+    seqs = [(3000, 20), (2048, 30)]
+    cache, q, offsets, keys, values = make(seqs, 4, 4, 128, 16, "float16", seed=4)
+    wide = torch.cat([q[:3], q, q[:5]])
+    out = torch.full_like(wide, 7.0)
+    cache.prefill(wide, offsets + 3, out=out)
+    for _ in range(20):
+        cache.prefill(wide, offsets + 3, out=out)
+    first = out.clone()
+    check(first[3:-5], q, offsets, keys, values, seqs, "float16")
+    assert bool((first[:3] == 7).all()) and bool((first[-5:] == 7).all())
+    shifted = offsets + 3
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            cache.prefill(wide, shifted, out=out)
+    out.fill_(7.0)
+    for _ in range(5):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)
+
+
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
 @pytest.mark.parametrize("window,sinks", MASKS)
 @pytest.mark.parametrize("seqs,heads,group,d,page", [
     ([(1, 1), (64, 1), (65, 1), (0, 1), (1000, 1), (127, 1), (2, 1)], 2, 4, 128, 16),
