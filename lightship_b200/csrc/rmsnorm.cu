@@ -10,8 +10,8 @@
 // where every buffer is 16-byte aligned and the length a multiple of 8, single elements elsewhere.
 // Longer rows are walked twice by one CTA.
 //
-// Measured: 16384 x 8192 bf16 with a residual in 185 us (5.80 TB/s); 12288 x 768 f32 to int8 in 22 us
-// (25 with a scale per row), which its 47 MB let the caches hold in part; one row of 4096 in 2.6 us.
+// Measured: 16384 x 8192 bf16 with a residual in 185 us (5.80 TB/s); 131072 x 768 f32 to int8 with a
+// scale per row in 131 us (3.84 TB/s); 8192 x 16384 bf16 in 106 us (5.07 TB/s); a row of 4096 in 3 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -118,35 +118,64 @@ __device__ __forceinline__ void store(T* p, const float (&f)[V]) {
 // The row's scale from its largest |y|: find_scale_zp's symmetric rule.
 __device__ __forceinline__ float row_scale(float top) { return top > 0.0f ? __fdiv_rn(top, 127.0f) : 1.0f; }
 
+// How the rows are worked on: CTAs that fit an SM by their registers, and whether a row is read while
+// the one before it is reduced and written (by CTAs that all run at once).  That keeps reads in flight
+// where few bytes per thread or one CTA per SM leave gaps (without and with it, us: 8192 x 16384 bf16 163 and 106, 300000 x 256 f16 84
+// and 64, 1000000 x 64 f16 70 and 53, 131072 x 768 f32 to int8 147 and 130); with two steps the registers
+// for it cost more than it gives (65536 x 2048 bf16 133 and 165, 32768 x 4096 f16 169 and 174).
+template <int V, int TPR, int STEPS>
+struct RowShape {
+  static constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
+  static constexpr int kCtas = V * STEPS <= 16 ? (TPR < 512 ? 4 : 2) : (TPR < 512 ? 2 : 1);
+  static constexpr bool kAhead = V == 8 && STEPS != 2;
+};
+
 // Rows in registers: TPR threads per row, STEPS steps of V elements per thread (element
 // (step * TPR + thread) * V).
 template <typename TX, typename TR, int V, int TPR, int STEPS>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, V * STEPS <= 16 ? (TPR < 512 ? 4 : 2) : (TPR < 512 ? 2 : 1))
+__global__ void __launch_bounds__(RowShape<V, TPR, STEPS>::kThreads, RowShape<V, TPR, STEPS>::kCtas)
     rmsnorm_rows_kernel(const RmsArgs a) {
-  constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR, kWarps = TPR / 32;
+  using Shape = RowShape<V, TPR, STEPS>;
+  constexpr int kThreads = Shape::kThreads, kRows = Shape::kRows, kWarps = TPR / 32;
+  constexpr bool kAhead = Shape::kAhead;
   __shared__ float red[2][kThreads / 32];
   griddep_wait();
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int in_row = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int d = static_cast<int>(a.d);
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kRows; r0 < a.rows; r0 += static_cast<int64_t>(gridDim.x) * kRows) {
-    const int64_t r = r0 + sub;
-    const bool live = r < a.rows;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  Raw<TX, V> xr[STEPS];
+  Raw<TR, V> rr[STEPS];
+  auto fetch = [&](int64_t r) {
     const TX* x = static_cast<const TX*>(a.x) + r * a.x_stride;
     const TR* res = static_cast<const TR*>(a.res) + r * a.res_stride;
-    Raw<TX, V> xr[STEPS];
-    Raw<TR, V> rr[STEPS];
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       const int i = (s * TPR + in_row) * V;
-      if (live && i < d) {
+      if (r < a.rows && i < d) {
         xr[s] = load<V>(x + i);
         if (a.res) rr[s] = load<V>(res + i);
       }
     }
+  };
+  if constexpr (kAhead) fetch(static_cast<int64_t>(blockIdx.x) * kRows + sub);
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kRows; r0 < a.rows; r0 += step) {
+    const int64_t r = r0 + sub;
+    const bool live = r < a.rows;
+    if constexpr (!kAhead) fetch(r);
     float h[STEPS][V];
     float ss = 0.0f, top = 0.0f;
+    auto count = [&](int s) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) ss = fmaf(h[s][e], h[s][e], ss);
+      if (a.row_scales) {
+        float g[V];
+        if (a.gamma) widen<V>(load<V>(a.gamma + (s * TPR + in_row) * V), g);
+#pragma unroll
+        for (int e = 0; e < V; ++e) top = fmaxf(top, fabsf(a.gamma ? h[s][e] * g[e] : h[s][e]));
+      }
+    };
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       const int i = (s * TPR + in_row) * V;
@@ -159,15 +188,14 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, V * STEPS <= 16 ? (TPR 
           for (int e = 0; e < V; ++e) h[s][e] = __fadd_rn(h[s][e], f[e]);
           if (a.sum_out) store<V>(static_cast<TR*>(a.sum_out) + r * a.sum_stride + i, h[s]);
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) ss = fmaf(h[s][e], h[s][e], ss);
-        if (a.row_scales) {
-          float g[V];
-          if (a.gamma) widen<V>(load<V>(a.gamma + i), g);
-#pragma unroll
-          for (int e = 0; e < V; ++e) top = fmaxf(top, fabsf(a.gamma ? h[s][e] * g[e] : h[s][e]));
-        }
+        if constexpr (!kAhead) count(s);
       }
+    }
+    if constexpr (kAhead) {
+      fetch(r + step);  // on its way while this row is reduced and written
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+        if (live && (s * TPR + in_row) * V < d) count(s);
     }
 #pragma unroll
     for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) {
@@ -289,9 +317,10 @@ __global__ void __launch_bounds__(kWalkThreads) rmsnorm_walk_kernel(const RmsArg
 
 template <typename TX, typename TR, int V, int TPR, int STEPS>
 lsc_status launch_rows(const RmsArgs& a, const DeviceState* ds, cudaStream_t st) {
-  constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
+  using Shape = RowShape<V, TPR, STEPS>;
+  constexpr int kThreads = Shape::kThreads, kRows = Shape::kRows;
   const int64_t ctas = (a.rows + kRows - 1) / kRows;
-  const int64_t cap = static_cast<int64_t>(ds->sm_count) * 32;
+  const int64_t cap = static_cast<int64_t>(ds->sm_count) * (Shape::kAhead ? Shape::kCtas : 32);
   LSC_CUDA_TRY(launch_dependent(ds->overlap_launches, rmsnorm_rows_kernel<TX, TR, V, TPR, STEPS>,
                                 dim3(static_cast<unsigned>(ctas < cap ? ctas : cap)), dim3(kThreads), 0, st, a));
   return LSC_SUCCESS;
@@ -300,7 +329,7 @@ lsc_status launch_rows(const RmsArgs& a, const DeviceState* ds, cudaStream_t st)
 template <typename TX, typename TR>
 lsc_status launch(const RmsArgs& a, const DeviceState* ds, bool vectors, cudaStream_t st) {
   // Few threads per row while they hold it in a few vectors, so that reductions stay within a warp and
-  // no lane idles: 12288 x 768 f32 to int8 took 30.9 us with 64 threads x 2 vectors and 22.3 with 32 x 3;
+  // no lane idles (measured before rows were read ahead): 12288 x 768 f32 to int8 took 30.9 us with 64 threads x 2 vectors and 22.3 with 32 x 3;
   // 100000 x 64 f16 took 26.9 with 32 threads and 9.5 with 8.  Single elements keep rows in registers
   // all the same: 16384 x 1001 f16 took 70 us when walked twice and 42.7 so.
   if (a.d <= kMaxRow && vectors) {

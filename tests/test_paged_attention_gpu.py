@@ -646,10 +646,10 @@ import sys, torch
 sys.path.insert(0, %r)
 from lightship_b200 import ops
 from lightship_b200.kv_cache import PagedKVCache
-k = torch.randn(40, 16, 2, 64, device="cuda").half()
+k = torch.randn(80, 16, 2, 64, device="cuda").half()
 v = torch.randn_like(k)
-lens = torch.tensor([600], dtype=torch.int32, device="cuda")
-cache = PagedKVCache(k, v, torch.arange(40, dtype=torch.int32, device="cuda")[None], lens)
+lens = torch.tensor([1200], dtype=torch.int32, device="cuda")
+cache = PagedKVCache(k, v, torch.arange(80, dtype=torch.int32, device="cuda")[None], lens)
 q = torch.randn(1, 4, 64, device="cuda").half()
 off = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
 new = torch.randn(1, 2, 64, device="cuda").half()
