@@ -25,8 +25,8 @@
 // that it follows are complete, because S of this tile was issued behind them.
 // What bounds it: 128 x 128 scores take 1024 clocks of the tensor cores with heads of 128 (both products) and
 // the same of the special function units, and a row tile's softmax and products follow one another; two row tiles
-// fill each other's gaps to 59 % of the tensor cores' measured rate.  Measured: 8192 tokens, 32 query
-// heads on 8 of 128 (f16) in 565 us, 974 TFLOP/s; 16 on 4 of 64 with a window of 1024 in 94 us; 100
+// fill each other's gaps to 60 % of the tensor cores' measured rate.  Measured: 8192 tokens, 32 query
+// heads on 8 of 128 (f16) in 555 us, 991 TFLOP/s; 16 on 4 of 64 with a window of 1024 in 94 us; 100
 // tokens of 12 heads of 64 in 7.7 us.
 // With few units (a chunk of a prompt on a long cache) a cluster of 2, 4 or 8 CTAs shares each of them:
 // every CTA takes a part of the unit's key tiles, keeps its own m, l and O, and sends each CTA of the
