@@ -496,6 +496,9 @@ lsc_status lsc_kv_cache_append(const lsc_paged_kv* cache, const void* k_new, con
  * Scores, maxima and sums in f32; probabilities are rounded to the cache's type for the second
  * product (as two such numbers where there is an int8 output, so that its codes are those of
  * unrounded ones; a value in V that is not finite leaves the codes of the rows it reaches open).
+ * f16 holds probabilities in steps no finer than 2^-31 of the row's largest (2^-39 for single tokens);
+ * bf16 has no such limit.
+ * A row whose every visible score is -infinity gives zeros.
  * out [tokens, q_heads, head_dim] contiguous in the cache's type and/or out_i8 of that shape,
  * quantized per tensor with s_out (`rounding` as lsc_rounding); 16-byte aligned.  Rows before the first offset or behind the last one are left
  * as they are.  What the cache holds behind a sequence's last token has no effect.  Rows are

@@ -73,6 +73,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return true;
 }
 
+// f16 ends at 2^16 above and rounds below 2^-14 in steps of 2^-24, so a probability taken relative to the
+// largest one would be lost from 2^-25 on, while the sum l still counts it: very many faint keys behind a
+// strong one would then shrink the output (131072 of them by 0.4 %).  So f16 probabilities, which reach
+// 2^MOST, go into the product with V times 2^kRaise, which brings those to 2^15.  bf16 has the exponents
+// of f32 and needs no factor.
+template <bool BF16, int MOST>
+constexpr int kRaise = BF16 ? 0 : 15 - MOST;
+
 // {lo, hi} rounded to the cache's type and packed
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {

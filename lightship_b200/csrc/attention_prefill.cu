@@ -20,8 +20,8 @@
 //                   sees (a product with p = 0 would keep a NaN) in the few tiles that have such
 //                   rows, before they are released to the products.
 // m moves only when a row's maximum passes it by more than 2^8: until then p stays below 2^8,
-// which the 16-bit types and the f32 sums hold as exactly as values below 1, and O needs no
-// rescaling.  When it moves, the softmax thread rescales its row of O in TMEM; the products into O
+// which bf16 and the f32 sums hold as exactly as values below 1, and O needs no rescaling.  In f16 all of
+// p, l and O carry a factor of 2^7 on top, so p stays below 2^15 and is not lost before 2^-32.  When it moves, the softmax thread rescales its row of O in TMEM; the products into O
 // that it follows are complete, because S of this tile was issued behind them.
 // What bounds it: 128 x 128 scores take 1024 clocks of the tensor cores with heads of 128 (both products) and
 // the same of the special function units, and a row tile's softmax and products follow one another; two row tiles
@@ -52,7 +52,7 @@ constexpr int kFirstPart = 96;
 // 503 us there, no turns at all 537.
 constexpr int kTurnAt = 3;
 constexpr int kSharedPlaces = 256;   // places per CTA of a cluster, at least
-constexpr float kMoveBy = 8.0f;  // log2 of how far a maximum may pass the reference
+constexpr int kMoveBy = 8;  // log2 of how far a maximum may pass the reference
 
 // max of three (NaN operands are ignored)
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           ref = m;
         } else {
           // also true where ref is -inf and m is not; false where both are
-          const bool move = (m - ref) * scale > kMoveBy;
+          const bool move = (m - ref) * scale > static_cast<float>(kMoveBy);
           if (__any_sync(0xffffffffu, move)) {
             if constexpr (Shape::kApart) {
               // The product of the tile before is complete when the next tile's scores, issued behind it,
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           }
         }
         ++done;
-        const float shift = ref == -INFINITY ? 0.0f : -ref * scale;
+        const float shift = ref == -INFINITY ? 0.0f : fmaf(-ref, scale, static_cast<float>(kRaise<BF16, kMoveBy>));
         const uint64_t scale2 = f2pack(scale, scale), shift2 = f2pack(shift, shift);
         uint64_t sum2[2] = {0ull, 0ull};
         // The two row tiles take turns at the special function units: in step with each other they would
