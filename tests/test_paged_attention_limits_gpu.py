@@ -79,3 +79,83 @@ def test_scores_just_below_a_move_of_the_reference(cuda, d, kind):
         cache.append(keys[0], values[0], offsets)
         check(cache.prefill(q, offsets, alpha=1.0), q, offsets, keys, values, [(n, n)], kind, alpha=1.0)
         check(cache.decode(q[-1:], alpha=1.0), q[-1:], torch.tensor([0, 1]), keys, values, [(n, 1)], kind, alpha=1.0)
+
+
+# ---- bad device data, shown on the whole buffers
+
+@pytest.mark.parametrize("case", ["negative length", "length past the table", "page past the cache", "negative page",
+                                  "offsets that decrease", "offset past the tokens", "more tokens than places"])
+def test_append_of_bad_device_data_writes_nothing_else(cuda, case):
+    """Guard pages on both sides of the cache: the well-formed sequences' places take their tokens, the bad
+    one's good places theirs, everything else stays to the bit, and the error word is raised."""
+    import torch
+    from lightship_b200 import _lib, ops
+    from lightship_b200._lib import LightShipError
+    from lightship_b200.kv_cache import PagedKVCache
+    page, heads, d, pages, guard, most = 16, 2, 64, 12, 5, 4
+    g = torch.Generator().manual_seed(3)
+    whole = [torch.randn(pages + 2 * guard, page, heads, d, generator=g).half().to(cuda) for _ in range(2)]
+    k, v = (w[guard:guard + pages] for w in whole)
+    table = torch.tensor([[3, 8, 1, -1], [10, 0, 5, 11], [7, 2, 4, -1]], dtype=torch.int32)
+    lens, offs = [40, 50, 30], [0, 40, 90, 120]
+    if case == "negative length":
+        lens[1] = -5
+    elif case == "length past the table":
+        lens[1] = 1 << 30
+    elif case == "page past the cache":
+        table[1, 0] = pages
+    elif case == "negative page":
+        table[1, 1] = -1
+    elif case == "offsets that decrease":
+        offs[1], offs[2] = 90, 40
+    elif case == "offset past the tokens":
+        offs[3] = 5000
+    else:
+        lens[1] = 20
+    tokens = 120
+    new = [torch.randn(tokens, heads, d, generator=g).half().to(cuda) for _ in range(2)]
+    want = [w.clone() for w in whole]
+    for b in range(3):
+        begin, end = offs[b], offs[b + 1]
+        if not 0 <= begin <= end <= tokens:
+            continue
+        n = min(max(lens[b], 0), most * page)
+        for t in range(begin, end):
+            p = n - (end - begin) + t - begin
+            if p < 0 or not 0 <= int(table[b, p // page]) < pages:
+                continue
+            at = guard + int(table[b, p // page])
+            for w, x in zip(want, new):
+                w[at, p % page] = x[t]
+    cache = PagedKVCache(k, v, table.to(cuda), torch.tensor(lens, dtype=torch.int32, device=cuda))
+    ops.check_device()
+    cache.append(new[0], new[1], torch.tensor(offs, dtype=torch.int32, device=cuda))
+    with pytest.raises(LightShipError) as e:
+        ops.check_device()
+    assert e.value.code == _lib.ERROR_EXECUTION_FAILED
+    for got, w in zip(whole, want):
+        assert torch.equal(got.view(torch.int16), w.view(torch.int16))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_infinite_scores(cuda, d):
+    """A key that scores -inf drops out; one that scores +inf makes NaN of the rows that see it and of no
+    other."""
+    import torch
+    n, at = 300, 37
+    for sign in (-1.0, 1.0):
+        cache, q, offsets, keys, values = make([(n, n)], 1, 2, d, 16, "float16", seed=6)
+        q.abs_().clamp_(min=0.01)
+        cache.k[int(cache.page_table[0, at // 16]), at % 16, 0, 5] = sign * math.inf
+        out, one = cache.prefill(q, offsets), cache.decode(q[-1:])
+        if sign > 0:
+            assert bool(out[at:].isnan().all()) and bool(one.isnan().all())
+            check(out[:at], q[:at], torch.tensor([0, at]), [keys[0][:at]], [values[0][:at]], [(at, at)], "float16")
+            continue
+        left = [i for i in range(n) if i != at]
+        rows = torch.cat([out[:at], out[at + 1:]])  # the row of the place itself sees the keys before it
+        qs = torch.cat([q[:at], q[at + 1:]])
+        off = torch.tensor([0, n - 1])
+        check(rows, qs, off, [keys[0][left]], [values[0][left]], [(n - 1, n - 1)], "float16")
+        check(out[at:at + 1], q[at:at + 1], torch.tensor([0, 1]), [keys[0][:at]], [values[0][:at]], [(at, 1)], "float16")
+        check(one, q[-1:], torch.tensor([0, 1]), [keys[0][left]], [values[0][left]], [(n - 1, 1)], "float16")
