@@ -159,3 +159,51 @@ def test_infinite_scores(cuda, d):
         check(rows, qs, off, [keys[0][left]], [values[0][left]], [(n - 1, n - 1)], "float16")
         check(out[at:at + 1], q[at:at + 1], torch.tensor([0, 1]), [keys[0][:at]], [values[0][:at]], [(at, 1)], "float16")
         check(one, q[-1:], torch.tensor([0, 1]), [keys[0][left]], [values[0][left]], [(n - 1, 1)], "float16")
+
+
+# ---- what a call takes does not hang on the table's width or on empty slots
+
+def _time(call):
+    """us a call: the best of several replays of twenty captured ones."""
+    import torch
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(20):
+            call()
+    best = math.inf
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    for _ in range(15):
+        begin.record()
+        graph.replay()
+        end.record()
+        torch.cuda.synchronize()
+        best = min(best, begin.elapsed_time(end) * 1e3 / 20)
+    return best
+
+
+@pytest.mark.parametrize("live", [[0, 1, 2, 3], [0, 700, 2000, 4095], [4092, 4093, 4094, 4095], [31, 32, 64, 1000]])
+@pytest.mark.parametrize("longest", [200, 3000])
+def test_decode_of_a_batch_padded_with_empty_slots(cuda, longest, live):
+    """Four sequences among 4096 slots: the values, zeros for the others, and a time that does not follow
+    where the empty slots are."""
+    import torch
+    slots = 4096
+    lens = {b: n for b, n in zip(live, [longest, 100, 1, longest - 50])}
+    seqs = [(lens.get(b, 0), 1) for b in range(slots)]
+    cache, q, offsets, keys, values = make(seqs, 2, 4, 128, 16, "float16", seed=live[1])
+    out = torch.full_like(q, 9.0)
+    ws = cache.decode_workspace(8)
+    cache.decode(q, out=out, workspace=ws)
+    rows = torch.tensor(live, device=cuda)
+    check(out[rows], q[rows], torch.arange(5), [keys[b] for b in live], [values[b] for b in live],
+          [seqs[b] for b in live], "float16")
+    out[rows] = 0.0
+    assert bool((out == 0).all())
+    packed = cache.kv_lens.clone()
+    took = _time(lambda: cache.decode(q, out=out, workspace=ws))
+    cache.kv_lens.zero_()
+    cache.kv_lens[-4:] = packed[rows]
+    cache.page_table[-4:] = cache.page_table[rows].clone()
+    assert took <= 2 * _time(lambda: cache.decode(q, out=out, workspace=ws))
