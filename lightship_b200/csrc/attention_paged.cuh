@@ -117,10 +117,11 @@ struct TileList {
     i += skip;
     return i < sink_tiles ? i : start + i - sink_tiles;
   }
-  // part x of `parts` equal ones
-  __device__ __forceinline__ void take(int32_t x, int32_t parts) {
-    skip = static_cast<int32_t>(static_cast<int64_t>(n) * x / parts);
-    n = static_cast<int32_t>(static_cast<int64_t>(n) * (x + 1) / parts) - skip;
+  // part x of `parts` equal ones (a few: a list of a sequence's 2^30 places has at most 2^24 tiles)
+  __device__ __forceinline__ void take(uint32_t x, uint32_t parts) {
+    const uint32_t all = static_cast<uint32_t>(n);
+    skip = static_cast<int32_t>(all * x / parts);
+    n = static_cast<int32_t>(all * (x + 1) / parts) - skip;
   }
 };
 

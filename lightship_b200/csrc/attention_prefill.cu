@@ -28,7 +28,7 @@
 // fill each other's gaps to 60 % of the tensor cores' measured rate.  Measured: 8192 tokens, 32 query
 // heads on 8 of 128 (f16) in 555 us, 991 TFLOP/s; 16 on 4 of 64 with a window of 1024 in 94 us; 100
 // tokens of 12 heads of 64 in 7.7 us.
-// With few units (a chunk of a prompt on a long cache) a cluster of 2, 4 or 8 CTAs shares each of them:
+// With few units (a chunk of a prompt on a long cache) a cluster of 2, 4 or 8 CTAs shares each long one:
 // every CTA takes a part of the unit's key tiles, keeps its own m, l and O, and sends each CTA of the
 // cluster a share of O's columns through distributed shared memory; the shares are joined there in
 // the order of the parts.  No workspace, no second launch.
@@ -51,7 +51,11 @@ constexpr int kFirstPart = 96;
 // The quarter of the exponentials after which the other row tile may begin: 1, 2 and 3 took 573, 546 and
 // 503 us there, no turns at all 537.
 constexpr int kTurnAt = 3;
-constexpr int kSharedPlaces = 256;   // places per CTA of a cluster, at least
+// Key tiles per CTA of a cluster that shares a unit, at least, and those of a unit from which on it is
+// shared.  A cluster's exchange takes about 6 us, a tile 1.6.  Whole and shared, us, with 8 units: 512 places
+// 13.0 and (2 parts) 13.5, 1024 places 19.4 and (4) 14.7, 4096 places 57 and (8) 22.5, 65536 places 807
+// and 121.
+constexpr int kPartTiles = 2, kSharedTiles = 8;
 constexpr int kMoveBy = 8;  // log2 of how far a maximum may pass the reference
 
 // max of three (NaN operands are ignored)
@@ -339,8 +343,18 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   };
   auto tiles_of = [&](const Unit& u) {
     TileList<kTile> tiles(u.pos0, u.pos0 + u.count - 1, a.window, a.sinks);
-    if (p.parts > 1) tiles.take(static_cast<int32_t>(blockIdx.x % p.parts), p.parts);
+    if (p.parts > 1) {
+      const uint32_t most = static_cast<uint32_t>(p.parts), part = blockIdx.x % most;
+      const uint32_t room = tiles.n < kSharedTiles ? 1 : static_cast<uint32_t>(tiles.n) / kPartTiles;
+      if (part < room) tiles.take(part, room < most ? room : most);
+      else tiles.n = 0;
+    }
     return tiles;
+  };
+  // The host knows the table's width only: what a cluster does with its unit goes by the unit's own tiles.
+  // Few of them belong to the first CTA alone, which writes the rows as a CTA without a cluster does.
+  auto is_shared = [&](const Unit& u) {
+    return TileList<kTile>(u.pos0, u.pos0 + u.count - 1, a.window, a.sinks).n >= kSharedTiles;
   };
 
   if (warp >= 8) {
@@ -819,7 +833,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
         }
         if (done >= 2) last_phase ^= 1u;
       }
-      if (p.parts > 1) break;
+      if (p.parts > 1 && (blockIdx.x % p.parts > 0 || is_shared(u))) break;
       const float inv = l == 0.0f ? 0.0f : __frcp_rn(l);
       const int64_t at = (static_cast<int64_t>(u.row0 + w * p.tpt + token) * a.q_heads + u.head0 + head) * D;
 #pragma unroll 1
@@ -865,7 +879,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       __syncwarp();
       cluster_sync();  // every CTA's products and copies are complete
       u = sched[0];
-      const bool here = u.b >= 0 && *abort_flag == 0u;
+      const bool here = u.b >= 0 && *abort_flag == 0u && is_shared(u);
       if (here && w == 0) {
         for (uint32_t x = 0; x < parts; ++x)
           asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(
@@ -1003,11 +1017,10 @@ lsc_status launch_prefill(const lsc_paged_kv* cache, const DeviceState* ds, cons
   int64_t places = static_cast<int64_t>(c.max_pages) << c.page_shift;
   const int64_t seen = static_cast<int64_t>(a.window) + a.sinks + p.tpt;
   if (a.window > 0 && places > seen) places = seen;
-  // A cluster's exchange takes about 6 us, a tile of 128 keys 1.6.  Whole and shared, us, with 8 units:
-  // 512 places 13.0 and (2 parts) 13.5, 1024 places 19.4 and (4) 14.7, 4096 places 57 and (8) 22.5, 65536
-  // places 807 and 121.  More clusters than run at once would take twice the time.
-  if (p.unit_tokens == p.tpt && places >= 1024) {
-    while (p.parts < 8 && 2 * p.parts * kSharedPlaces <= places) {
+  // As many CTAs as the longest sequence that the table has room for could use; more clusters than run at
+  // once would take twice the time.
+  if (p.unit_tokens == p.tpt && places >= kSharedTiles * kTile) {
+    while (p.parts < 8 && 2 * p.parts * kPartTiles * kTile <= places) {
       int fit = 0;
       if ((s = clusters_at_once<BF16, D, FINE>(2 * p.parts, &fit))) return s;
       if (most > fit) break;

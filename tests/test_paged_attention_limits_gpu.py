@@ -207,3 +207,49 @@ def test_decode_of_a_batch_padded_with_empty_slots(cuda, longest, live):
     cache.kv_lens[-4:] = packed[rows]
     cache.page_table[-4:] = cache.page_table[rows].clone()
     assert took <= 2 * _time(lambda: cache.decode(q, out=out, workspace=ws))
+
+
+def _widened(cache, places):
+    """The same cache under a table of `places` per sequence."""
+    import torch
+    from lightship_b200.kv_cache import PagedKVCache
+    page = cache.k.shape[1]
+    table = torch.full((cache.batch, places // page), -1, dtype=torch.int32, device=cache.device)
+    table[:, :cache.page_table.shape[1]] = cache.page_table[:, :places // page]
+    return PagedKVCache(cache.k, cache.v, table, cache.kv_lens)
+
+
+def test_short_prompts_under_a_wide_table(cuda):
+    """A table with room for 8192 places a sequence: the rows are those of a fitted table, to the bit, and the
+    call does not pay for a cluster's exchange (7.4, 8.5 and 10.5 us fitted; 9.1, 10.8 and 13.5 wide; with the
+    exchange 11.3, 13.7 and 15.3)."""
+    import torch
+    took = [0.0, 0.0]
+    for kind, n, heads, group, d, page in (("float16", 100, 12, 1, 64, 16), ("float16", 100, 8, 4, 128, 64),
+                                           ("bfloat16", 256, 8, 4, 128, 64)):
+        cache, q, offsets, keys, values = make([(n, n)], heads, group, d, page, kind, seed=n)
+        wide = _widened(cache, 8192)
+        outs = [torch.full_like(q, 9.0) for _ in range(2)]
+        codes = [torch.full(q.shape, 99, dtype=torch.int8, device=cuda) for _ in range(2)]
+        for i, c in enumerate((cache, wide)):
+            c.prefill(q, offsets, out=outs[i], out_i8=codes[i], s_out=0.02)
+            took[i] += _time(lambda: c.prefill(q, offsets, out=outs[i]))
+        check(outs[1], q, offsets, keys, values, [(n, n)], kind)
+        assert torch.equal(codes[0], codes[1])
+        wide.prefill(q, offsets, out=outs[1])
+        assert torch.equal(outs[0], outs[1])
+    assert took[1] <= 1.4 * took[0], took
+
+
+@pytest.mark.parametrize("kind", ["float16", "bfloat16"])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (900, 3), (3000, 0)])
+def test_short_and_long_units_of_one_call(cuda, window, sinks, kind):
+    """Clusters that share their unit beside such that leave it to one CTA: 7, 8, 9 and 15 key tiles, one, none."""
+    from lightship_b200 import ops
+    seqs = [(896, 30), (897, 30), (1024, 9), (1025, 1), (1152, 7), (1920, 33), (5, 5), (1, 1), (0, 0), (0, 3), (6000, 12)]
+    for heads, group, d in ((1, 2, 64), (1, 4, 128)):
+        cache, q, offsets, keys, values = make(seqs, heads, group, d, 16, kind, seed=d)
+        wide = _widened(cache, 65536)
+        for c in (cache, wide):
+            check(c.prefill(q, offsets, window=window, sinks=sinks), q, offsets, keys, values, seqs, kind, window, sinks)
+    ops.check_device()
