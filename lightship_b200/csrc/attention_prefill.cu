@@ -33,10 +33,10 @@
 // cluster a share of O's columns through distributed shared memory; the shares are joined there in
 // the order of the parts.  No workspace, no second launch.
 // Every wait is bounded (a timeout flags the device error word and ends the CTA's work).
-#include <mutex>
 #include <type_traits>
 
 #include "attention_paged.cuh"
+#include "device_count.h"
 
 namespace lsc {
 namespace {
@@ -956,30 +956,26 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   }
 }
 
-// Clusters of so many CTAs (2, 4 or 8) that the device runs at the same time
+// Whether the device runs `units` clusters of 2, 4 or 8 CTAs at the same time; no, where it does not say.
 template <bool BF16, int D, bool FINE>
-lsc_status clusters_at_once(int cluster, int* fit) {
-  static std::once_flag once;
-  static cudaError_t failed = cudaSuccess;
-  static int known[9];
-  std::call_once(once, [] {
-    for (int n = 2; n <= 8 && failed == cudaSuccess; n *= 2) {
-      cudaLaunchConfig_t cfg = {};
-      cudaLaunchAttribute attr[1];
-      attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = static_cast<unsigned>(n);
-      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-      cfg.gridDim = dim3(static_cast<unsigned>(n));
-      cfg.blockDim = dim3(kPrefillThreads);
-      cfg.dynamicSmemBytes = PrefillShape<D, FINE>::kSmem;
-      cfg.attrs = attr;
-      cfg.numAttrs = 1;
-      failed = cudaOccupancyMaxActiveClusters(known + n, paged_prefill_kernel<BF16, D, FINE>, &cfg);
-    }
+bool clusters_fit(const DeviceState* ds, int cluster, int64_t units) {
+  static DeviceCount counts[3];
+  const int at_once = counts[cluster / 4].get(ds->device, [&](int* n) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(cluster));
+    cfg.blockDim = dim3(kPrefillThreads);
+    cfg.dynamicSmemBytes = PrefillShape<D, FINE>::kSmem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const bool known = cudaOccupancyMaxActiveClusters(n, paged_prefill_kernel<BF16, D, FINE>, &cfg) == cudaSuccess;
+    if (!known) cudaGetLastError();  // the call goes on without clusters
+    return known;
   });
-  if (failed != cudaSuccess) return cuda_error(failed, "paged_attention_prefill: clusters");
-  *fit = known[cluster];
-  return LSC_SUCCESS;
+  return units <= at_once;
 }
 
 template <bool BF16, int D, bool FINE>
@@ -1020,12 +1016,9 @@ lsc_status launch_prefill(const lsc_paged_kv* cache, const DeviceState* ds, cons
   // As many CTAs as the longest sequence that the table has room for could use; more clusters than run at
   // once would take twice the time.
   if (p.unit_tokens == p.tpt && places >= kSharedTiles * kTile) {
-    while (p.parts < 8 && 2 * p.parts * kPartTiles * kTile <= places) {
-      int fit = 0;
-      if ((s = clusters_at_once<BF16, D, FINE>(2 * p.parts, &fit))) return s;
-      if (most > fit) break;
+    while (p.parts < 8 && 2 * p.parts * kPartTiles * kTile <= places &&
+           clusters_fit<BF16, D, FINE>(ds, 2 * p.parts, most))
       p.parts *= 2;
-    }
   }
   if (p.parts > 1) grid = static_cast<int>(most) * p.parts;  // units of one row tile: there are few
   LSC_CUDA_TRY(launch_clusters(ds->overlap_launches, paged_prefill_kernel<BF16, D, FINE>, dim3(grid),

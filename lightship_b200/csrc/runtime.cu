@@ -7,6 +7,7 @@
 
 #include <mutex>
 
+#include "device_count.h"
 #include "lsc_internal.h"
 #include "sm100.cuh"
 
@@ -19,7 +20,6 @@ thread_local char t_last_error[1024] = "";
 // device in device_state) and atomically OR LSC_DEVERR_* bits into it.
 __device__ uint32_t g_device_error_word;
 
-constexpr int kMaxDevices = 64;
 std::mutex g_state_mu;
 DeviceState g_states[kMaxDevices];
 bool g_state_ready[kMaxDevices] = {};
