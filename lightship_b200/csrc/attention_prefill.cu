@@ -150,11 +150,16 @@ struct Scheduler {
   int32_t top;
   // What is known of sequence b: its rows, its length, its units and their first level.
   struct Seq {
-    int32_t begin, count, len, n, base;
+    int32_t b, begin, count, len, n, base;
   };
-  Seq held;  // of sequence `lane`: batches of up to 32 are read once
+  // Up to 32 sequences with new tokens are held by a lane each, and what follows never reads the batch again
+  // (slots: 32); else the batch is read each time (slots: its size) and the first 32 are held.  Four
+  // prompts that take 76 us alone take 87 in a batch of 1024 slots so, and took 167 to 195 without the list.
+  Seq held;
+  int slots;
   __device__ __forceinline__ Seq read(int b) const {
     Seq s{};
+    s.b = b;
     if (b >= c.batch) return s;
     int32_t end;
     query_rows(p.a.offsets, b, p.a.tokens, c.err, false, s.begin, end);
@@ -164,11 +169,36 @@ struct Scheduler {
     s.base = s.len > s.count ? (s.len - s.count) / p.unit_tokens : 0;
     return s;
   }
-  __device__ __forceinline__ Seq of(int b) const { return b == lane ? held : read(b); }
+  __device__ __forceinline__ Seq of(int i) const { return i == lane ? held : read(i); }
+  __device__ __forceinline__ void hold() {
+    held = read(lane);
+    slots = c.batch;
+    if (c.batch <= 32) return;
+    Seq list{};
+    int live = 0;
+#pragma unroll 1
+    for (int b = 0; b < c.batch; b += 32) {
+      const Seq s = read(b + lane);
+      for (uint32_t mask = __ballot_sync(0xffffffffu, s.n > 0); mask; mask &= mask - 1) {
+        const int src = __ffs(mask) - 1;
+        Seq t;
+        t.b = b + src;
+        t.begin = __shfl_sync(0xffffffffu, s.begin, src);
+        t.count = __shfl_sync(0xffffffffu, s.count, src);
+        t.len = __shfl_sync(0xffffffffu, s.len, src);
+        t.n = __shfl_sync(0xffffffffu, s.n, src);
+        t.base = __shfl_sync(0xffffffffu, s.base, src);
+        if (live == 32) return;
+        if (lane == live++) list = t;
+      }
+    }
+    held = list;
+    slots = 32;
+  }
   __device__ __forceinline__ int64_t at_or_above(int32_t t) const {
     int64_t f = 0;
 #pragma unroll 1
-    for (int b = lane; b < c.batch; b += 32) {
+    for (int b = lane; b < slots; b += 32) {
       const Seq s = of(b);
       const int32_t x = s.base + s.n - t;
       f += x < 0 ? 0 : (x > s.n ? s.n : x);
@@ -179,9 +209,9 @@ struct Scheduler {
   }
   __device__ __forceinline__ Scheduler(const PagedView& c_, const PrefillArgs& p_, int lane_)
       : c(c_), p(p_), lane(lane_), top(0) {
-    held = read(lane);
+    hold();
 #pragma unroll 1
-    for (int b = lane; b < c.batch; b += 32) {
+    for (int b = lane; b < slots; b += 32) {
       const Seq s = of(b);
       top = s.n > 0 && s.base + s.n > top ? s.base + s.n : top;
     }
@@ -225,7 +255,7 @@ struct Scheduler {
     const int32_t k = static_cast<int32_t>(u - above);
     Unit r{};
 #pragma unroll 1
-    for (; scan_b < c.batch; scan_b += 32) {
+    for (; scan_b < slots; scan_b += 32) {
       const Seq s = of(scan_b + lane);
       const bool here = s.base <= level && level < s.base + s.n;
       const uint32_t mask = __ballot_sync(0xffffffffu, here);
@@ -238,7 +268,7 @@ struct Scheduler {
       for (int x = scan_k; x < k; ++x) rest &= rest - 1;
       const int src = __ffs(rest) - 1;
       const int32_t first = (level - s.base) * p.unit_tokens;
-      r.b = scan_b + src;
+      r.b = __shfl_sync(0xffffffffu, s.b, src);
       r.row0 = __shfl_sync(0xffffffffu, s.begin + first, src);
       r.count = __shfl_sync(0xffffffffu, s.count - first < p.unit_tokens ? s.count - first : p.unit_tokens, src);
       r.pos0 = __shfl_sync(0xffffffffu, s.len - s.count + first, src);
@@ -361,12 +391,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     regs_shrink<88>();
     if (warp == 10) {
       // ------------------------------------------------------------------ units, zeroing of unseen V rows
-      if (blockIdx.x == 0) {
+      // the CTAs share the check of the batch
+#pragma unroll 1
+      for (int64_t b = blockIdx.x * 32 + lane; b < c.batch; b += gridDim.x * 32) {
         int32_t begin, end;
-        for (int b = lane; b < c.batch; b += 32) {
-          query_rows(a.offsets, b, a.tokens, c.err, true, begin, end);
-          paged_len(c, b, true);
-        }
+        query_rows(a.offsets, static_cast<int>(b), a.tokens, c.err, true, begin, end);
+        paged_len(c, static_cast<int>(b), true);
       }
       Scheduler s(c, p, lane);
       int64_t round = 0;         // of the next unit to find: the grid walks them to and fro
