@@ -138,7 +138,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
   constexpr int kRows = 16 * MT;
   constexpr int kBlocks = D / 64;           // 128-byte column blocks of a row
   constexpr int kStages = Shape::kStages;
-  constexpr float kUp = 1 << kRaise<BF16, 0>, kDown = 1.0f / kUp;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
   float* swap = reinterpret_cast<float*>(smem + kStages * 2 * Shape::kTileBytes);
@@ -397,6 +396,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
         ref[r] = now == -INFINITY ? 0.0f : now;
         f[r] = ex2_approx(m[r] - ref[r]);
         m[r] = now;
+        ref[r] -= kRaise<BF16, 0>;
       }
       if (__any_sync(0xffffffffu, f[0] != 1.0f || f[1] != 1.0f)) {
         l[0] *= f[0];
@@ -409,8 +409,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
           o[n][3] *= f[1];
         }
       }
-      // p = 2^(s - m), rounded to the cache's type for the product with V (the sums take it unrounded); in
-      // f16 as 2^15 p, an exact factor that O gives back when it is written
+      // p = 2^(s - m), rounded to the cache's type for the product with V (the sums take it unrounded).  In
+      // f16 all of p, l and O carry a factor of 2^15, here and where parts are joined.
 #pragma unroll
       for (int n = 0; n < kKeys / 16; ++n) {
         float e[8];
@@ -419,7 +419,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
           const int r = (x >> 1) & 1;
           e[x] = ex2_approx(s[2 * n + (x >> 2)][x & 3] - ref[r]);
           l[r] += e[x];
-          e[x] *= kUp;
         }
         const uint32_t pa[4] = {pack16<BF16>(e[0], e[1]), pack16<BF16>(e[2], e[3]), pack16<BF16>(e[4], e[5]),
                                 pack16<BF16>(e[6], e[7])};
@@ -472,15 +471,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2)
       swap_phase ^= 1u;
       return ok;
     };
-    if constexpr (kUp != 1.0f) {
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        o[n][0] *= kDown;
-        o[n][1] *= kDown;
-        o[n][2] *= kDown;
-        o[n][3] *= kDown;
-      }
-    }
     float top[2] = {m[0], m[1]};
     if constexpr (kSlices > 1) {
       if ((lane & 3) == 0) {
