@@ -438,7 +438,8 @@ lsc_status lsc_attention_f16(const void* qkv, int64_t batch, int64_t seq, int64_
  * rows (>= d); the elements of a row are contiguous.  Any d, strides and alignment to the
  * element's size; rows that are 16-byte aligned throughout are read as vectors.  sum_out may be
  * residual or x itself, out may be x itself (same type and stride); no other overlap.  A row
- * whose sum of squares overflows f32 gives zeros. */
+ * whose sum of squares overflows f32 gives zeros; with eps = 0 one whose sum of squares is 0 or underflows
+ * gives NaN where h is 0 and infinities elsewhere. */
 lsc_status lsc_rmsnorm(const void* x, int32_t x_dtype, int64_t x_stride, const void* residual,
                        int32_t residual_dtype, int64_t residual_stride, int64_t rows, int64_t d,
                        const float* gamma, float eps, void* sum_out, int64_t sum_stride, void* out,
@@ -494,8 +495,9 @@ lsc_status lsc_kv_cache_append(const lsc_paged_kv* cache, const void* k_new, con
  * tokens stay visible.  A row that sees no key (p < 0) gives zeros.
  *   out[t, h, :] = softmax_j(alpha * q . k_j) v_j       alpha > 0
  * Scores, maxima and sums in f32; probabilities are rounded to the cache's type for the second
- * product (as two such numbers where there is an int8 output, so that its codes are those of
- * unrounded ones; a value in V that is not finite leaves the codes of the rows it reaches open).
+ * product, as two such numbers where there is an int8 output: of its codes about one in 10^4 (prompts on
+ * a bf16 cache) to 10^5 differs by one from that of the exact value, next to a border.  There a value in
+ * V that is not finite leaves the codes of the rows it reaches open.
  * f16 holds probabilities in steps no finer than 2^-31 of the row's largest (2^-39 for single tokens);
  * bf16 has no such limit.
  * A row whose every visible score is -infinity gives zeros.

@@ -3,8 +3,8 @@
 //   O[b, h, :] = sum_j p_j V[j, :] / l,  p_j = 2^(s_j - m),  s_j = alpha log2(e) Q[b, h, :] . K[j, :]
 // with m the running maximum and l the sum of p over the visible places j.
 //
-// Every byte of K and V is read once and used for at most 4 flops per query head of its group, so
-// the cache's bandwidth bounds it.  The work is cut by bytes, not by sequences: the key tiles (64
+// Every byte of K and V is read once (once per 64 heads of a larger group) and used for at most 4 flops per
+// query head of its group, so the cache's bandwidth bounds it.  The work is cut by bytes, not by sequences: the key tiles (64
 // places) of all (sequence, key-value head) pairs form one list, and CTA c of G takes tiles
 // [c T / G, (c + 1) T / G) of it, so a ragged batch and a single long sequence load the GPU alike.
 // A CTA meets whole pairs, which it writes out itself, and at most two cut ones (its first and its
@@ -16,8 +16,12 @@
 // Four warps multiply: the up to 16 query heads of a group are the rows of m16n8k16 products (the
 // instruction needs one eighth of the rows that tcgen05 does, and at 4 flops a byte the legacy
 // tensor path is far from its limit).  Measured: 131072 places of 8 bf16 heads of 128, 32 query heads, in
-// 92 us (5.83 TB/s of keys and values); 64 sequences of up to 8192 places in 183 us (5.95 TB/s).  Groups of more than 16 heads give the warps heads instead
-// of keys: MT row tiles x (4 / MT) key slices.  Each warp keeps its own m, l and O.
+// 92 to 94 us (5.7 to 5.8 TB/s of keys and values); 64 sequences of up to 8192 places in 182 to 195 us
+// (5.6 to 6.0 TB/s).  Groups of more than 16 heads give the warps heads instead of keys: MT row tiles x
+// (4 / MT) key slices.  Each warp keeps its own m, l and O.  With heads of 128 that takes more registers
+// than there are: two row tiles spill about 90 bytes a thread and four about 290 (350 for an int8
+// output), and every warp reads the keys of its slice for itself (16 sequences of 4096 places, 64 heads on
+// one, 31 us; its bytes alone would take 5).
 #include "attention_paged.cuh"
 
 namespace lsc {

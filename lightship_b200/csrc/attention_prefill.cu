@@ -25,9 +25,11 @@
 // that it follows are complete, because S of this tile was issued behind them.
 // What bounds it: 128 x 128 scores take 1024 clocks of the tensor cores with heads of 128 (both products) and
 // the same of the special function units, and a row tile's softmax and products follow one another; two row tiles
-// fill each other's gaps to 60 % of the tensor cores' measured rate.  Measured: 8192 tokens, 32 query
-// heads on 8 of 128 (f16) in 555 us, 991 TFLOP/s; 16 on 4 of 64 with a window of 1024 in 94 us; 100
-// tokens of 12 heads of 64 in 7.7 us.
+// fill each other's gaps to 60 to 70 % of the tensor cores' measured rate.  Measured: 8192 tokens, 32 query
+// heads on 8 of 128 (f16) in 555 to 565 us, 985 TFLOP/s, call after call (the power limit lowers the clock),
+// and in 475 in bursts of a few calls at 1965 MHz, which is how the figures beside the rules below were
+// taken; 16 on 4 of 64 with a window of 1024 in 95 us; 100 tokens of 12 heads of 64 in 7.7 us.  An int8
+// output takes 1.3 times as long (475 and 617 us), for the second product with V.
 // With few units (a chunk of a prompt on a long cache) a cluster of 2, 4 or 8 CTAs shares each long one:
 // every CTA takes a part of the unit's key tiles, keeps its own m, l and O, and sends each CTA of the
 // cluster a share of O's columns through distributed shared memory; the shares are joined there in
@@ -46,14 +48,14 @@ constexpr int kPrefillThreads = 384;
 constexpr int kSchedSlots = 4;
 constexpr int kParts = 2;        // parts of P that are passed on
 // Keys of the first part.  The products of the last part are what the next scores wait for, so it is
-// small; 64 keys took 510 us where 96 take 497 (8192 tokens, 32 query heads on 8 of 128).
+// small; 64 keys took 477 us where 96 take 474 (8192 tokens, 32 query heads on 8 of 128).
 constexpr int kFirstPart = 96;
-// The quarter of the exponentials after which the other row tile may begin: 1, 2 and 3 took 573, 546 and
-// 503 us there, no turns at all 537.
+// The quarter of the exponentials after which the other row tile may begin: 1, 2 and 3 took 476, 475 and
+// 474 us there, no turns at all 490.
 constexpr int kTurnAt = 3;
 // Key tiles per CTA of a cluster that shares a unit, at least, and those of a unit from which on it is
 // shared.  A cluster's exchange takes about 6 us, a tile 1.6.  Whole and shared, us, with 8 units: 512 places
-// 13.0 and (2 parts) 13.5, 1024 places 19.4 and (4) 14.7, 4096 places 57 and (8) 22.5, 65536 places 807
+// 13.0 and (2 parts) 13.5, 1024 places 19.5 and (4) 14.7, 4096 places 57 and (8) 22.6, 65536 places 810
 // and 121.
 constexpr int kPartTiles = 2, kSharedTiles = 8;
 constexpr int kMoveBy = 8;  // log2 of how far a maximum may pass the reference
@@ -1034,8 +1036,8 @@ lsc_status launch_prefill(const lsc_paged_kv* cache, const DeviceState* ds, cons
                                     Shape::kSmem));
   // Two row tiles per unit hide one's softmax behind the other's products; with fewer units than SMs
   // one row tile each spreads the work over more of them.  One and two, us: 256 tokens of 12 heads of 64
-  // 8.7 and 9.6; 32 query heads on 8 of 128, 512 tokens 14.6 and 16.2, 1024 tokens (136 units) 25.1 and
-  // 24.3, 2048 tokens 66.9 and 42.8.
+  // 9.1 and 10.1; 32 query heads on 8 of 128, 512 tokens 15.2 and 16.5, 1024 tokens (136 units) 25.8 and
+  // 25.5, 2048 tokens 68.4 and 44.9.
   p.unit_tokens = units(2 * p.tpt) < ds->sm_count ? p.tpt : 2 * p.tpt;
   const int64_t most = units(p.unit_tokens);
   int grid = static_cast<int>(most < ds->sm_count ? most : ds->sm_count);

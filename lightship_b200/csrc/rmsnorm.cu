@@ -10,8 +10,10 @@
 // where every buffer is 16-byte aligned and the length a multiple of 8, single elements elsewhere.
 // Longer rows are walked twice by one CTA.
 //
-// Measured: 16384 x 8192 bf16 with a residual in 185 us (5.80 TB/s); 131072 x 768 f32 to int8 with a
-// scale per row in 131 us (3.84 TB/s); 8192 x 16384 bf16 in 106 us (5.07 TB/s); a row of 4096 in 3 us.
+// Measured: with a residual, 16384 x 8192 bf16 in 183 to 192 us (5.6 to 5.9 TB/s) and 131072 x 768 f32 to
+// int8 with a scale per row in 206 us (6.4 TB/s); without one, where fewer bytes are in flight, 130 us
+// (3.9 TB/s) for the same rows to int8, 8192 x 16384 bf16 105 us (5.1 TB/s) and 65536 x 2048 bf16 133 us
+// (4.0 TB/s); single elements, 131072 x 1001 f16, 255 us (2.1 TB/s); a row of 4096 2.5 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -120,9 +122,13 @@ __device__ __forceinline__ float row_scale(float top) { return top > 0.0f ? __fd
 
 // How the rows are worked on: CTAs that fit an SM by their registers, and whether a row is read while
 // the one before it is reduced and written (by CTAs that all run at once).  That keeps reads in flight
-// where few bytes per thread or one CTA per SM leave gaps (without and with it, us: 8192 x 16384 bf16 163 and 106, 300000 x 256 f16 84
-// and 64, 1000000 x 64 f16 70 and 53, 131072 x 768 f32 to int8 147 and 130); with two steps the registers
-// for it cost more than it gives (65536 x 2048 bf16 133 and 165, 32768 x 4096 f16 169 and 174).
+// where few bytes per thread or one CTA per SM leave gaps; with two steps the registers for it cost more
+// than it gives.  Without and with it, us, for rows without a residual and (with one): 8192 x 16384 bf16
+// 162 and 105 (198 and 182), 300000 x 256 f16 84 and 63 (111 and 96), 1000000 x 64 f16 69 and 52 (92 and
+// 81), 131072 x 768 f32 to int8 147 and 130 (205 and 206); two steps, 65536 x 2048 bf16 133 and 165 (178
+// and 188), 32768 x 4096 f16 121 and 150 (169 and 175).  The two-step kernels spill all the same, 8 to 56
+// bytes a thread in 16 bits and about 120 in f32, as do <f32, 512 x 4> (144) and single elements,
+// <256 x 16> (52).
 template <int V, int TPR, int STEPS>
 struct RowShape {
   static constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
